@@ -94,6 +94,8 @@ _SIGNATURES = {
     "bx_logp_rowmax": (I, [P, L, P, P, I, I, P]),
     "bx_logp_rowsum": (I, [P, L, P, P, I, P, P, I, I, I, P]),
     "bx_logp_finish": (I, [P, P, P, P, I, I, P]),
+    "bx_log_probs": (I, [I, P, L, P, I, P, P, P, P, P, I, I, I, P]),
+    "bx_step_tables": (I, [P, P, P, P, L, I, I, P, I, P, I, I, P, P, P, P, P, P, P, I, P]),
 }
 
 
@@ -226,6 +228,15 @@ def ptr(t):
 def stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def here(*tensors):
+    """Refuses tensors of the host, or of another device than the current one, whose stream the kernels go to."""
+    import torch
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
 
 
 def device_status():

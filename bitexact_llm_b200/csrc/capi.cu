@@ -20,6 +20,8 @@
 #include "prefill_attention.cuh"
 #include "sampler.cuh"
 #include "logp.cuh"
+#include "logprobs.cuh"
+#include "step_tables.cuh"
 #include "decompose.cuh"
 #include "unfused.cuh"
 #include "unfused_stages.cuh"
@@ -444,6 +446,24 @@ int exact_linear_auto(int M, int N, int K, bool residual) {
   const int forms[3] = {664, 648, -48};
   const int best = cost[0] <= cost[1] && cost[0] <= cost[2] ? 0 : cost[1] <= cost[2] ? 1 : 2;
   return 100 * cost[best] < 99 * given ? forms[best] : form;
+}
+
+// CTAs that share a row: as many as fill the SMs several times over while a CTA still reads 32 KB.
+int log_probs_cluster(int M, int V, int bytes) {
+  int c = 1;
+  while (c < LP_MAX_CLUSTER && (long long)M * c < 4ll * 4 * device_sms() && (long long)V * bytes / (2 * c) >= 32768) c *= 2;
+  return c;
+}
+
+template <class T, bool TOP>
+int launch_log_probs(const LogProbs& a, int M, cudaStream_t st) {
+  static PerDevice configured;
+  if (once_per_device(configured, [] {
+        return cudaFuncSetAttribute(log_probs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      }) != BX_OK)
+    return BX_ELAUNCH;
+  const int c = log_probs_cluster(M, a.V, sizeof(T));
+  return launch_chained(log_probs_kernel<T, TOP>, dim3((unsigned)M * c), LP_THREADS, sizeof(LpShared<typename LpOf<T>::Val>), st, c, a);
 }
 
 }  // namespace
@@ -1796,6 +1816,47 @@ int bx_exact_linear_static(const int32_t* q, int64_t ldq, const int64_t* sh, con
   }
   return bx_exact_linear(q, ldq, sh, limbs, d, g, cnt, ec, ev, R, planes, y, flag, M, N, K, checked, tile_rows,
                          stream);
+}
+
+// ---- log probabilities ----
+int bx_log_probs(int kind, const void* logits, int64_t ld, const int64_t* tok, int top, float* logp, float* entropy, int64_t* rank,
+                 int64_t* top_ids, float* top_logp, int M, int V, int fr, void* stream) {
+  if (g_status_seen.load(std::memory_order_relaxed)) return BX_EDEVICE;
+  if (kind < 0 || kind > 2 || M < 0 || V < 1 || ld < V || top < 0 || fr < 0 || fr > 40) return BX_EARG;
+  if (top > LP_MAX_TOP || M > (1 << 26) || V > (1 << 30)) return BX_ELIMIT;
+  if (M == 0) return BX_OK;
+  if (!logits || !entropy || (tok && (!logp || !rank)) || (top && (!top_ids || !top_logp)) || !aligned_to(logits, kind == BX_LOGITS_I64 ? 8 : kind == BX_LOGITS_F32 ? 4 : 2))
+    return BX_EARG;
+  const int shift = fr > 24 ? fr - 24 : 0;
+  const LogProbs a{logits, ld, reinterpret_cast<const long long*>(tok), V, top, shift, 1.0f / (float)(1ll << (fr - shift)), logp, entropy,
+                   reinterpret_cast<long long*>(rank), reinterpret_cast<long long*>(top_ids), top_logp};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (kind == BX_LOGITS_I64) return top ? launch_log_probs<long long, true>(a, M, st) : launch_log_probs<long long, false>(a, M, st);
+  if (kind == BX_LOGITS_F32) return top ? launch_log_probs<float, true>(a, M, st) : launch_log_probs<float, false>(a, M, st);
+  return top ? launch_log_probs<__nv_bfloat16, true>(a, M, st) : launch_log_probs<__nv_bfloat16, false>(a, M, st);
+}
+
+// ---- tables of a step ----
+int bx_step_tables(const int64_t* lens, const int64_t* counts, const uint8_t* drop, int32_t* bt, int64_t bt_stride, int nblk, int page,
+                   int32_t* free, int pool, int32_t* top, int B, int rows, int64_t* seq, int64_t* pos, int64_t* slot, int64_t* last,
+                   int64_t* lens_out, int32_t* top_out, int32_t* status, int sticky, void* stream) {
+  if (g_status_seen.load(std::memory_order_relaxed)) return BX_EDEVICE;
+  if (B < 0 || rows < 0 || nblk < 1 || page < 1 || pool < 0 || bt_stride < nblk) return BX_EARG;
+  if (B > ST_MAX_REQUESTS || (long long)nblk * page > 0x3fffffff || (long long)B * nblk > 0x7fffffff || rows > (1 << 30)) return BX_ELIMIT;
+  if (!top || !top_out || !status || (B && (!lens || !counts || !bt || !last || !lens_out)) || (pool && !free) ||
+      (rows && (!seq || !pos || !slot)))
+    return BX_EARG;
+  static PerDevice configured;
+  if (once_per_device(configured, [] {
+        return cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * ST_MAX_REQUESTS);
+      }) != BX_OK)
+    return BX_ELAUNCH;
+  // a CTA for every two rows of a thread
+  int c = 1;
+  while (c < ST_MAX_CLUSTER && rows > 2 * ST_THREADS * c) c *= 2;
+  const StepTables a{(const long long*)lens, (const long long*)counts, drop, bt, bt_stride, free, top, status, (long long*)seq, (long long*)pos,
+                     (long long*)slot, (long long*)last, (long long*)lens_out, top_out, B, nblk, page, pool, rows, sticky};
+  return launch_chained(step_tables_kernel, dim3(c), ST_THREADS, 16 * B, (cudaStream_t)stream, c, a);
 }
 
 }  // extern "C"

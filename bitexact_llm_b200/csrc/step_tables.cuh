@@ -1,0 +1,153 @@
+// The tables of a step's token rows from the requests' lengths, on the device: pages of finished requests go back to the pool, new
+// ones are taken from it, and every row gets its request, position and cache slot.
+//
+// The pool is a stack of page numbers. Request b holds ceil(len / page) pages. Dropped requests push theirs in the order of the
+// requests, a request's last page first; then every request takes ceil((len + n) / page) - ceil(len / page) pages, in the order of
+// requests and positions. Nothing is taken or given back when something does not fit: the status tells what.
+//
+// One cluster of CTAs. Each CTA scans all requests' counts for itself (rows, pages pushed, pages taken: the running sums stay in
+// shared memory), then rows and pages are dealt over all threads, which find their request by bisection: even work whatever the
+// lengths. Inputs are read before the cluster's barrier and outputs written behind it, so that they may be the same memory. What
+// bounds it is latency: a chain of three dependent loads (length, page of the table or the stack, store).
+#pragma once
+
+#include "bx_ptx.cuh"
+
+namespace bx {
+
+constexpr int ST_THREADS = 1024, ST_MAX_REQUESTS = 8192, ST_MAX_CLUSTER = 8;
+
+struct StepTables {
+  const long long *lens, *counts;
+  const uint8_t* drop;                                     // NULL: no request is finished
+  int* bt;
+  long long bt_stride;
+  int *free, *top, *status;
+  long long *seq, *pos, *slot, *last, *lens_out;
+  int* top_out;
+  int B, nblk, page, pool, rows, sticky;
+};
+
+// First index of ends[0 .. n - 1] (non-decreasing) whose value exceeds i.
+__device__ __forceinline__ int st_owner(const int* ends, int n, int i) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > i) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int st_pages(long long n, int page) { return (int)((n + page - 1) / page); }
+
+__global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTables a) {
+  extern __shared__ int st_smem[];
+  int* row_end = st_smem;                                  // running sums, [B] each
+  int* push_end = row_end + a.B;
+  int* take_end = push_end + a.B;
+  int* base = take_end + a.B;                              // a request's length before its new tokens
+  __shared__ long long warp_rows[32];
+  __shared__ int warp_push[32], warp_take[32], bad_bits;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t rank, ctas;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+  if (tid == 0) bad_bits = 0;
+  launch_next();
+  wait_previous();
+  const long long most = (long long)a.nblk * a.page;
+  const int top = *a.top;
+  long long rows = 0;
+  int push = 0, take = 0;
+  for (int b0 = 0; b0 < a.B; b0 += ST_THREADS) {
+    const int b = b0 + tid;
+    long long n = 0;
+    int gone = 0, need = 0, start = 0, bad = 0;
+    if (b < a.B) {
+      const long long len = a.lens[b];
+      n = a.counts[b];
+      const bool out = a.drop && a.drop[b];
+      if (len < 0 || n < 0 || len > most) bad = BX_STEP_INVALID;
+      else if ((out ? 0 : len) > most - n) bad = BX_STEP_TOO_LONG;
+      if (bad) n = 0;
+      else {
+        start = out ? 0 : (int)len;
+        gone = out ? st_pages(len, a.page) : 0;
+        need = st_pages(start + n, a.page) - st_pages(start, a.page);
+      }
+    }
+    long long r = n;
+    int p = gone, t = need;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long r2 = __shfl_up_sync(0xffffffffu, r, o);
+      const int p2 = __shfl_up_sync(0xffffffffu, p, o), t2 = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) r += r2, p += p2, t += t2;
+    }
+    __syncthreads();                                       // bad_bits is set, the sums of the requests before are read
+    if (bad) atomicOr(&bad_bits, bad);
+    if (lane == 31) warp_rows[warp] = r, warp_push[warp] = p, warp_take[warp] = t;
+    __syncthreads();
+    long long all_r = rows;
+    int all_p = push, all_t = take;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      if (w == warp) r += all_r, p += all_p, t += all_t;
+      all_r += warp_rows[w], all_p += warp_push[w], all_t += warp_take[w];
+    }
+    if (b < a.B) {
+      row_end[b] = (int)min(r, 0x7fffffffll);
+      push_end[b] = p;
+      take_end[b] = t;
+      base[b] = start;
+    }
+    rows = all_r, push = all_p, take = all_t;
+  }
+  __syncthreads();
+  int bad = bad_bits;
+  if (top < 0 || top > a.pool - push) bad |= BX_STEP_INVALID;
+  else if (take > top + push) bad |= BX_STEP_NO_PAGES;
+  if (rows > a.rows) bad |= BX_STEP_TOO_MANY_ROWS;
+  const int at = rank * ST_THREADS + tid, step = ctas * ST_THREADS;
+  if (!bad)
+    for (int i = at; i < push; i += step) {
+      const int b = st_owner(push_end, a.B, i);
+      a.free[top + i] = a.bt[b * a.bt_stride + push_end[b] - 1 - i];
+    }
+  __threadfence();
+  cluster_arrive();
+  cluster_wait();
+  const int full = top + push;
+  if (rank == 0) {
+    for (int b = tid; b < a.B; b += ST_THREADS) {
+      const int n = row_end[b] - (b ? row_end[b - 1] : 0);
+      if (!bad) a.lens_out[b] = base[b] + n;
+      else if (a.lens_out != a.lens) a.lens_out[b] = a.lens[b];
+      a.last[b] = !bad && n > 0 ? row_end[b] - 1 : -1;
+    }
+    if (tid == 0) {
+      *a.top_out = bad ? top : full - take;
+      *a.status = a.sticky ? *a.status | bad : bad;
+    }
+  }
+  const volatile int* stack = a.free;                      // another CTA of the cluster may have pushed
+  if (!bad)
+    for (int i = at; i < take; i += step) {
+      const int b = st_owner(take_end, a.B, i);
+      const int nth = i - (b ? take_end[b - 1] : 0);
+      a.bt[b * a.bt_stride + st_pages(base[b], a.page) + nth] = stack[full - 1 - i];
+    }
+  for (int i = at; i < a.rows; i += step) {
+    if (bad || i >= rows) {
+      a.seq[i] = 0, a.pos[i] = 0, a.slot[i] = -1;
+      continue;
+    }
+    const int b = st_owner(row_end, a.B, i), pos = base[b] + i - (b ? row_end[b - 1] : 0);
+    const int held = st_pages(base[b], a.page), block = pos / a.page;
+    const int page = block < held ? a.bt[b * a.bt_stride + block] : stack[full - 1 - (b ? take_end[b - 1] : 0) - (block - held)];
+    a.seq[i] = b, a.pos[i] = pos, a.slot[i] = (long long)page * a.page + pos % a.page;
+  }
+}
+
+}  // namespace bx

@@ -1,0 +1,89 @@
+"""The block table and the token rows of a step, kept and made on the device (`bx_step_tables`): a decode step that takes pages as its
+sequences grow needs no host synchronisation and can be captured into a CUDA graph.
+
+`step_tables` is the operator; `DevicePages` holds the state of a pool (lengths, table, stack of free pages) and steps it in place.
+`decode.Session(..., pages=n, on_device=True)` serves from one."""
+
+from typing import NamedTuple
+
+import torch
+
+from . import _native as nv
+
+TOO_LONG, NO_PAGES, TOO_MANY_ROWS, INVALID = 1, 2, 4, 8
+MAX_REQUESTS = 8192
+
+
+class StepTables(NamedTuple):
+    seq: torch.Tensor           # int64 [rows]: request of every new token, in order
+    pos: torch.Tensor           # int64 [rows]
+    slot: torch.Tensor          # int64 [rows]: cache slot; the places behind the last token are (0, 0, -1)
+    last: torch.Tensor          # int64 [B]: row of a request's last new token, -1 where it has none
+    lens: torch.Tensor          # int64 [B]: the lengths behind the step
+    top: torch.Tensor           # int32 [1]: free pages behind the step
+    status: torch.Tensor        # int32 [1]: 0, or why nothing was done
+
+
+def step_tables(lens, counts, bt, free, top, page, rows, drop=None, lens_out=None, top_out=None, status=None):
+    """lens, counts int64 [B]: tokens in the cache and new ones; bt int32 [B, blocks] (extended in place); free int32 [pool], top
+    int32 [1]: the stack of free pages, of which the first `top` are there (its end is written in place); rows: token rows that the
+    step has room for; drop bool [B] or None: requests that are over give their pages back first, and begin anew if they have new tokens.
+
+    lens_out, top_out: where the state behind the step goes (may be lens and top; default: new tensors, so that the same call again
+    gives the same rows). status: an int32 [1] to which this call's bits are added (default: a new one). Bits: TOO_LONG, NO_PAGES,
+    TOO_MANY_ROWS, INVALID; with any of them no page changes hands and all rows are padding."""
+    B = lens.shape[0] if lens.dim() == 1 else -1
+    if any(t.dtype != torch.int64 or t.shape != (B,) or not t.is_contiguous() for t in (lens, counts, *(() if lens_out is None else (lens_out,)))):
+        raise ValueError("step_tables: lens and counts int64 [B], contiguous")
+    if bt.dtype != torch.int32 or bt.dim() != 2 or bt.shape[0] != B or bt.shape[1] < 1 or bt.shape[1] > 1 and bt.stride(1) != 1 or B > 1 and bt.stride(0) < bt.shape[1]:
+        raise ValueError("step_tables: bt int32 [B, blocks], rows contiguous")
+    if free.dtype != torch.int32 or free.dim() != 1 or not free.is_contiguous():
+        raise ValueError("step_tables: free int32 [pool], contiguous")
+    if any(t.dtype != torch.int32 or t.numel() != 1 for t in (top, *(t for t in (top_out, status) if t is not None))):
+        raise ValueError("step_tables: top and status int32 [1]")
+    if drop is not None and (drop.dtype != torch.bool or drop.shape != (B,) or not drop.is_contiguous()):
+        raise ValueError("step_tables: drop bool [B], contiguous")
+    if page < 1 or rows < 0 or B > MAX_REQUESTS:
+        raise ValueError(f"step_tables: pages of at least one token, at most {MAX_REQUESTS} requests")
+    nv.here(lens, counts, bt, free, top, drop, lens_out, top_out, status)
+    dev = lens.device
+    seq, pos, slot = torch.empty(3, rows, dtype=torch.int64, device=dev).unbind(0)
+    last = torch.empty(B, dtype=torch.int64, device=dev)
+    lens_out = torch.empty_like(lens) if lens_out is None else lens_out
+    top_out = torch.empty_like(top) if top_out is None else top_out
+    sticky = status is not None
+    status = status if sticky else torch.empty(1, dtype=torch.int32, device=dev)
+    rc = nv.lib().bx_step_tables(lens.data_ptr(), counts.data_ptr(), nv.ptr(drop), bt.data_ptr(), bt.stride(0) if B > 1 else bt.shape[1],
+                                 bt.shape[1], page, free.data_ptr(), free.shape[0], top.data_ptr(), B, rows, seq.data_ptr(), pos.data_ptr(),
+                                 slot.data_ptr(), last.data_ptr(), lens_out.data_ptr(), top_out.data_ptr(), status.data_ptr(), int(sticky),
+                                 nv.stream())
+    nv.check(rc, "bx_step_tables")
+    return StepTables(seq, pos, slot, last, lens_out, top_out, status)
+
+
+class DevicePages:
+    """A pool of `pages` pages (numbers from 1 on, in the order of `order` when given) for B requests of up to `blocks` pages each."""
+
+    def __init__(self, B, blocks, pages, page, dev, order=None):
+        self.page = page
+        self.lens = torch.zeros(B, dtype=torch.int64, device=dev)
+        self.bt = torch.zeros(B, blocks, dtype=torch.int32, device=dev)
+        order = torch.arange(1, pages + 1) if order is None else order
+        self.free = order.flip(0).to(torch.int32).to(dev)
+        self.top = torch.full((1,), pages, dtype=torch.int32, device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def step(self, counts, rows, drop=None):
+        """One step in place: counts int64 [B] new tokens on at most `rows` rows. -> StepTables."""
+        return step_tables(self.lens, counts, self.bt, self.free, self.top, self.page, rows, drop, self.lens, self.top, self.status)
+
+    def check(self):
+        """Raises what a step found since the last check (synchronises)."""
+        bits = int(self.status)
+        self.status.zero_()
+        if bits & NO_PAGES:
+            raise MemoryError("the session has no free pages")
+        if bits & TOO_LONG:
+            raise ValueError("a sequence has more tokens than its row of the block table holds (max_len)")
+        if bits:
+            raise ValueError("a step had more new tokens than rows" if bits & TOO_MANY_ROWS else "a step's lengths or pages are not valid")

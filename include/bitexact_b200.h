@@ -534,6 +534,39 @@ int bx_logp_rowsum(const int64_t* logits, int64_t ld, const int64_t* rowmax, con
                    void* scratch, int64_t* S, int M, int V, int fr, void* stream);
 int bx_logp_finish(const int64_t* S, const int64_t* zt, const int64_t* lnt, int64_t* out, int M, int fr, void* stream);
 
+/* Log probabilities of rows of logits [M, V] (row stride ld >= V): BX_LOGITS_I64 fixed point at fr bits (0 .. 40; an entry of at most
+ * -2^62 is masked), BX_LOGITS_F32, BX_LOGITS_BF16 (-infinity is masked; fr unused). With p = softmax(row):
+ *   tok int64 [M] (NULL: none given; logp and rank are then not written): logp float [M] = ln p[tok] (-infinity where tok is masked,
+ *     NaN where it is outside [0, V)), rank int64 [M] = 1 + the entries above tok's + the equal ones at lower indices (0 where outside)
+ *   entropy float [M] = -sum p ln p
+ *   top (0 .. BX_MAX_TOP): top_ids int64 [M, top], top_logp float [M, top], the best entries in order, equal ones by index; where a
+ *     row has fewer unmasked entries the rest is (-1, -infinity).
+ * A row with NaN or +infinity, or without an unmasked entry, has NaN, rank 0 and ids -1. Sums in 32 bits, the same bits in every call. */
+#define BX_LOGITS_I64 0
+#define BX_LOGITS_F32 1
+#define BX_LOGITS_BF16 2
+#define BX_MAX_TOP 32
+int bx_log_probs(int kind, const void* logits, int64_t ld, const int64_t* tok, int top, float* logp, float* entropy, int64_t* rank,
+                 int64_t* top_ids, float* top_logp, int M, int V, int fr, void* stream);
+
+/* The tables of a step on the device. Request b (of B <= 8192) has lens[b] tokens in the cache, on pages bt[b][0 .. ceil(lens / page))
+ * (bt int32 [B, nblk], row stride bt_stride), and counts[b] >= 0 new ones. free int32 [pool] is a stack of page numbers, top int32 [1]
+ * their number. drop uint8 [B] (NULL: none): a request that is over gives its pages back first (in the order of requests, its last
+ * page first) and goes on, if counts says so, as a new one from length 0. Then the requests take the pages that their new tokens need
+ * from the end of the stack, in the order of requests and positions; bt is extended in place.
+ *   seq, pos, slot int64 [rows]: request, position and cache slot (page number * page + pos % page) of every new token, requests in
+ *     order; the places behind the last token get (0, 0, -1)
+ *   last int64 [B]: the row of a request's last new token (-1: none); lens_out int64 [B], top_out int32 [1]: the state behind the
+ *     step (may be lens and top themselves)
+ *   status int32 [1]: the bits below, ORed to those that are there if sticky. When any is due, nothing is taken or given back: rows are all padding, lens_out = lens. */
+#define BX_STEP_TOO_LONG 1        /* a request has more tokens than its row of the table holds */
+#define BX_STEP_NO_PAGES 2        /* the pool has too few pages */
+#define BX_STEP_TOO_MANY_ROWS 4   /* more new tokens than rows */
+#define BX_STEP_INVALID 8         /* a negative length or count, a length beyond the table, a stack that does not fit the pool */
+int bx_step_tables(const int64_t* lens, const int64_t* counts, const uint8_t* drop, int32_t* bt, int64_t bt_stride, int nblk, int page,
+                   int32_t* free, int pool, int32_t* top, int B, int rows, int64_t* seq, int64_t* pos, int64_t* slot, int64_t* last,
+                   int64_t* lens_out, int32_t* top_out, int32_t* status, int sticky, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
