@@ -7,6 +7,7 @@
 #include "../../include/bitexact_float.h"
 #include "host_util.cuh"
 #include "fl_attention.cuh"
+#include "fl_attention4.cuh"
 #include "fl_attention_tc.cuh"
 #include "fl_gemm.cuh"
 #include "fl_gemm_simt.cuh"
@@ -293,6 +294,27 @@ int run_attention(int dtype, const PagedAttn& a, void* scratch, size_t scratch_b
   if (dtype == BXF_F32) fl_paged_attention_kernel<float><<<grid, LA_THREADS, a.W * 4, st>>>(a);
   else fl_paged_attention_kernel<bf16><<<grid, LA_THREADS, a.W * 4, st>>>(a);
   return launched(1);
+}
+
+bool cache4_ok(const void* cache, int kv_heads, int dim, int vdim, int page, int nb) {
+  return cache && kv_heads >= 1 && dim >= 1 && vdim >= 1 && page >= 1 && page % C4_TOKENS == 0 && nb >= 1 && aligned16(cache);
+}
+
+Cache4 cache4_of(const void* cache, int kv_heads, int dim, int vdim, int page, int nb) {
+  return {static_cast<uint8_t*>(const_cast<void*>(cache)), nb, kv_heads, page, dim, vdim, ceil_div(dim, 64) * 64, ceil_div(vdim, 64) * 64};
+}
+
+// Many rows: 32 to a CTA, so that the bytes of their values leave together; few: a CTA for every four.
+template <class T>
+int launch_store4(const Store4<T>& a, cudaStream_t st) {
+  if (a.M <= 512)
+    return launch_chained(fl_store4_kernel<T, 4>, dim3(ceil_div(a.M, 4), a.c.G), S4_THREADS, 0, st, 0, a);
+  return launch_chained(fl_store4_kernel<T, 32>, dim3(ceil_div(a.M, 32), a.c.G), S4_THREADS, (a.c.V / 2 + a.c.V / 16 + 1) * 36, st, 0, a);
+}
+
+template <class T>
+int launch_attention4(const PagedAttn& a, const Cache4& c, int variant, cudaStream_t st) {
+  return launch_chained(fl_attention4_plain_kernel<T>, dim3(a.M, a.H * a.G), A4_THREADS, (c.K + 2 * c.V) * 4, st, 0, a, c);
 }
 
 bool gru_ok(const bxf_gru* g, int M, int width) {
@@ -630,6 +652,56 @@ int bxf_gqa_attention(int dtype, const void* q, int64_t ldq, int M, int heads, i
                     nblk, reinterpret_cast<const i64*>(seq), reinterpret_cast<const i64*>(pos), tiles, ntiles, window, sink,
                     scale, out, ldo, vdim};
   return run_attention(dtype, a, scratch, scratch_bytes, variant, stream_of(stream));
+}
+
+size_t bxf_cache4_block(int dim, int vdim) {
+  return dim < 1 || vdim < 1 ? 0 : (size_t)cache4_of(nullptr, 1, dim, vdim, C4_TOKENS, 1).bytes();
+}
+
+int bxf_gqa_store4(int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                   const int64_t* slot, int M, int kv_heads, int dim, int vdim, void* cache, int page, int nb, void* stream) {
+  if (!dtype_ok(dtype) || M < 0 || !cache4_ok(cache, kv_heads, dim, vdim, page, nb)) return BX_EARG;
+  if (dim > C4_MAX || vdim > C4_MAX || kv_heads > 65535) return BX_ELIMIT;
+  if (M == 0) return BX_OK;
+  if (!k || !v || !slot) return BX_EARG;
+  const Cache4 c = cache4_of(cache, kv_heads, dim, vdim, page, nb);
+  const i64* slot_ = reinterpret_cast<const i64*>(slot);
+  cudaStream_t st = stream_of(stream);
+  if (dtype == BXF_F32)
+    return launch_store4<float>({static_cast<const float*>(k), static_cast<const float*>(v), k_row, k_head, v_row, v_head, slot_, M, c}, st);
+  return launch_store4<bf16>({static_cast<const bf16*>(k), static_cast<const bf16*>(v), k_row, k_head, v_row, v_head, slot_, M, c}, st);
+}
+
+int bxf_gqa_read4(int dtype, const void* cache, int kv_heads, int dim, int vdim, int page, int nb, const int64_t* slot, void* k, void* v,
+                  int M, void* stream) {
+  if (!dtype_ok(dtype) || M < 0 || !cache4_ok(cache, kv_heads, dim, vdim, page, nb)) return BX_EARG;
+  if (dim > C4_MAX || vdim > C4_MAX || kv_heads > 65535) return BX_ELIMIT;
+  if (M == 0) return BX_OK;
+  if (!slot || !k || !v) return BX_EARG;
+  const Cache4 c = cache4_of(cache, kv_heads, dim, vdim, page, nb);
+  const i64* slot_ = reinterpret_cast<const i64*>(slot);
+  const dim3 grid(M, kv_heads);
+  cudaStream_t st = stream_of(stream);
+  if (dtype == BXF_F32)
+    return launch_chained(fl_read4_kernel<float>, grid, 128, 0, st, 0, c, slot_, static_cast<float*>(k), static_cast<float*>(v), M);
+  return launch_chained(fl_read4_kernel<bf16>, grid, 128, 0, st, 0, c, slot_, static_cast<bf16*>(k), static_cast<bf16*>(v), M);
+}
+
+int bxf_gqa_attention4(int dtype, const void* q, int64_t ldq, int M, int heads, int kv_heads, int dim, int vdim, const void* cache, int page,
+                       int nb, const void* bt, int bt_is64, int64_t bt_stride, int nblk, const int64_t* seq, const int64_t* pos,
+                       const int* tiles, int ntiles, int window, const float* sink, float scale, void* out, int64_t ldo, int variant,
+                       void* stream) {
+  if (!dtype_ok(dtype) || M < 0 || heads < 1 || !cache4_ok(cache, kv_heads, dim, vdim, page, nb) || heads % kv_heads || ldq < dim ||
+      ldo < (int64_t)heads * vdim || nblk < 1 || window < 0 || ntiles < 0 || variant < 0 || variant > 2)
+    return BX_EARG;
+  if (dim > C4_MAX || vdim > C4_MAX || heads > 65535 || (i64)nblk * page > 0x3fffffff) return BX_ELIMIT;
+  if (g_status_seen.load() != 0) return BX_EDEVICE;
+  if (M == 0) return BX_OK;
+  if (!q || !bt || !seq || !pos || !out) return BX_EARG;
+  const Cache4 c = cache4_of(cache, kv_heads, dim, vdim, page, nb);
+  const PagedAttn a{q, ldq, M, heads / kv_heads, kv_heads, dim, vdim, 0, cache, c.bytes(), page, nb, bt, bt_is64, bt_stride, nblk,
+                    reinterpret_cast<const i64*>(seq), reinterpret_cast<const i64*>(pos), tiles, ntiles, window, sink, scale, out, ldo, vdim};
+  return dtype == BXF_F32 ? launch_attention4<float>(a, c, variant, stream_of(stream)) : launch_attention4<bf16>(a, c, variant, stream_of(stream));
 }
 
 int bxf_streams(int dtype, const bxf_streams_step* p, int M, void* stream) {

@@ -213,6 +213,77 @@ def gqa_attention(q, spec, cache, bt, seq, pos, sink, tiles=None, variant=0):
     return out
 
 
+CACHE4_TOKENS = 64              # pages of the 4-bit cache are multiples of this
+
+
+def gqa_cache4(spec, n_blocks, page, dev):
+    """An empty cache of keys and values in 4 bits (its form: include/bitexact_float.h) for pages of `page` tokens, a multiple of 64."""
+    if page < 1 or page % CACHE4_TOKENS:
+        raise ValueError(f"the 4-bit cache has pages of multiples of {CACHE4_TOKENS} tokens, not {page}")
+    return torch.zeros(n_blocks, spec.kv_heads, page // CACHE4_TOKENS, nv.float_lib().bxf_cache4_block(spec.dim, spec.vdim),
+                       dtype=torch.uint8, device=dev)
+
+
+def _check4(cache, dim, vdim):
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.shape[3] != nv.float_lib().bxf_cache4_block(dim, vdim):
+        raise ValueError(f"not a 4-bit cache for keys of {dim} and values of {vdim} entries")
+
+
+def gqa_store4(k, v, slot, cache):
+    """Rows of keys k T [M, kv_heads, dim] and values v T [M, kv_heads, vdim] (unit last stride) into the 4-bit cache at slot int64 [M]:
+    different slots; rows with a slot outside the cache (padding) are left out."""
+    M, G, dim = k.shape
+    if v.shape[:2] != (M, G) or k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float32) or cache.shape[1] != G:
+        raise ValueError("gqa_store4: keys and values of one type, a row of each for every token and head of the cache")
+    if slot.shape != (M,) or slot.dtype != torch.int64 or not slot.is_contiguous() or k.stride(2) != 1 and dim > 1 or v.stride(2) != 1 and v.shape[2] > 1:
+        raise ValueError("gqa_store4: slot int64 [M], rows of keys and values contiguous")
+    _check4(cache, dim, v.shape[2])
+    nv.here(k, v, slot, cache)
+    rc = nv.float_lib().bxf_gqa_store4(code(k), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slot.data_ptr(),
+                                       M, G, dim, v.shape[2], cache.data_ptr(), cache.shape[2] * CACHE4_TOKENS, cache.shape[0], nv.stream())
+    nv.check(rc, "bxf_gqa_store4")
+
+
+def gqa_read4(cache, spec, slot, dtype):
+    """-> the keys T [M, kv_heads, dim] and values T [M, kv_heads, vdim] that the 4-bit cache holds at slot int64 [M] (exact in bf16 too; zeros
+    for slots outside the cache)."""
+    M, G = slot.shape[0], cache.shape[1]
+    if slot.dtype != torch.int64 or slot.dim() != 1 or not slot.is_contiguous() or dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("gqa_read4: slot int64 [M], bfloat16 or float32")
+    _check4(cache, spec.dim, spec.vdim)
+    nv.here(slot, cache)
+    k, v = (torch.empty(M, G, n, dtype=dtype, device=cache.device) for n in (spec.dim, spec.vdim))
+    rc = nv.float_lib().bxf_gqa_read4(code(k), cache.data_ptr(), G, spec.dim, spec.vdim, cache.shape[2] * CACHE4_TOKENS, cache.shape[0],
+                                      slot.data_ptr(), k.data_ptr(), v.data_ptr(), M, nv.stream())
+    nv.check(rc, "bxf_gqa_read4")
+    return k, v
+
+
+def gqa_attention4(q, spec, cache, bt, seq, pos, sink, tiles=None, variant=0):
+    """`gqa_attention` over a 4-bit cache: q T [kv_heads, M, heads per group, ldq] -> T [M, pad8(heads vdim)]."""
+    G, M, per, ldq = q.shape
+    H, dim, vdim = spec.heads, spec.dim, spec.vdim
+    if cache.shape[1] != G or G * per != H or ldq < dim or q.dtype not in (torch.bfloat16, torch.float32) or not q.is_contiguous():
+        raise ValueError("gqa_attention4: queries T [kv_heads, M, heads per group, >= dim], contiguous")
+    if bt.dtype not in (torch.int32, torch.int64) or bt.dim() != 2 or bt.shape[1] > 1 and bt.stride(1) != 1:
+        raise ValueError("gqa_attention4: bt int32 or int64 [sequences, blocks], rows contiguous")
+    if any(t.dtype != torch.int64 or t.shape != (M,) or not t.is_contiguous() for t in (seq, pos)):
+        raise ValueError("gqa_attention4: seq and pos int64 [M]")
+    if tiles is not None and (tiles.dtype != torch.int32 or tiles.dim() != 2 or tiles.shape[1] != 3 or not tiles.is_contiguous()):
+        raise ValueError("gqa_attention4: tiles int32 [T, 3]")
+    if sink is not None and (sink.dtype != torch.float32 or sink.shape != (H,) or not sink.is_contiguous()):
+        raise ValueError("gqa_attention4: sink float32 [heads]")
+    _check4(cache, dim, vdim)
+    nv.here(q, cache, bt, seq, pos, sink, tiles)
+    out = torch.empty(M, pad8(H * vdim), dtype=q.dtype, device=q.device)
+    rc = nv.float_lib().bxf_gqa_attention4(code(q), q.data_ptr(), ldq, M, H, G, dim, vdim, cache.data_ptr(), cache.shape[2] * CACHE4_TOKENS,
+                                           cache.shape[0], bt.data_ptr(), int(bt.dtype == torch.int64), bt.stride(0), bt.shape[1],
+                                           seq.data_ptr(), pos.data_ptr(), nv.ptr(tiles), 0 if tiles is None else tiles.shape[0], spec.window,
+                                           nv.ptr(sink), spec.scale, out.data_ptr(), out.shape[1], variant, nv.stream())
+    nv.check(rc, "bxf_gqa_attention4")
+    return out
+
+
 def conv_of(u, w, b, state, step):
     """bxf_conv of inputs u T [M, channels] (a view into wider rows), w float [taps, channels]."""
     return nv.Conv(u=u.data_ptr(), ldu=u.stride(0), w=w.data_ptr(), b=b.data_ptr(), state=state.data_ptr(),

@@ -262,6 +262,29 @@ int bxf_gqa_attention(int dtype, const void* q, int64_t ldq, int M, int heads, i
                       int window, const float* sink, float scale, void* out, int64_t ldo, void* scratch,
                       size_t scratch_bytes, int variant, void* stream);
 
+/* Keys and values in 4 bits: cache uint8 [nb, kv_heads, page / 64, bxf_cache4_block(dim, vdim)], page a multiple of 64, 16-byte aligned,
+ * zero before its first use. With K and V = dim and vdim rounded up to multiples of 64, the block of 64 tokens of one head holds
+ *   key codes [64][K / 2] (entry 2 i in the low half of byte i) | key scales [4][2][K / 16][8] (token 16 a + 2 t + b, entries 16 j .. 16 j + 15
+ *   at [a][b][j][t]) | value codes [V / 16][8][64] (entry 16 j + i of a token in the low half of [j][i][token], 16 j + i + 8 in the high half) |
+ *   value scales [V / 16][64] | key exponents [64] | value exponents [64].
+ * An entry is code * scale * 2^(exponent - 127): code e2m1 (sign, 0 .5 1 1.5 2 3 4 6), scale e4m3. Of a row (a token's key or value of one head):
+ * exponent = floor(log2(largest magnitude)) - 10, within -100 .. 117; scale = the smallest of which 6 steps reach the largest of its 16
+ * entries; code = the nearest, ties to the even one. A row with NaN or an infinity in its key or value has NaN scales in its key and a
+ * value of zeros. Magnitudes beyond 2^127 are kept as 2^127. dim, vdim <= 512.
+ *   bxf_gqa_store4      k T [M][kv_heads] rows (strides k_row, k_head), v the same; slot int64 [M] (page * page size + token; different ones;
+ *                       rows with a slot outside the cache are left out)
+ *   bxf_gqa_read4       what the cache holds at slot: k T [M, kv_heads, dim], v T [M, kv_heads, vdim] (zeros for a slot outside)
+ *   bxf_gqa_attention4  as bxf_gqa_attention; variant 0 automatic, 1 the plain kernel. */
+size_t bxf_cache4_block(int dim, int vdim);
+int bxf_gqa_store4(int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                   const int64_t* slot, int M, int kv_heads, int dim, int vdim, void* cache, int page, int nb, void* stream);
+int bxf_gqa_read4(int dtype, const void* cache, int kv_heads, int dim, int vdim, int page, int nb, const int64_t* slot, void* k, void* v,
+                  int M, void* stream);
+int bxf_gqa_attention4(int dtype, const void* q, int64_t ldq, int M, int heads, int kv_heads, int dim, int vdim, const void* cache, int page,
+                       int nb, const void* bt, int bt_is64, int64_t bt_stride, int nblk, const int64_t* seq, const int64_t* pos,
+                       const int* tiles, int ntiles, int window, const float* sink, float scale, void* out, int64_t ldo, int variant,
+                       void* stream);
+
 int bxf_streams(int dtype, const bxf_streams_step* step, int M, void* stream);
 int bxf_causal_conv(int dtype, const bxf_conv* conv, void* out, int64_t ldo, int M, void* stream);
 int bxf_recurrence(int dtype, const bxf_recurrence_rows* rows, int M, void* stream);
