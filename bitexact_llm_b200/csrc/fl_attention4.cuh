@@ -3,6 +3,7 @@
 
 #include "fl_attention.cuh"
 #include "fl_cache4.cuh"
+#include "fl_gemm.cuh"
 
 namespace bxf {
 
@@ -84,6 +85,439 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
   T* o = static_cast<T*>(a.out) + m * a.out_tok + h * a.out_head;
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   for (int d = tid; d < a.R; d += A4_THREADS) st(o + d, (acc[d] + acc[c.V + d]) * inv);
+}
+
+// ---- bf16 queries, keys and values of 64 or 128 entries: matrix instructions on operands that are made in registers ----
+//
+// The cache rows are the M side: scores S^T = K Q^T and outputs O^T = V^T P^T by m16n8k16 with fp32 accumulators, the query rows (tokens
+// x heads of a group) being the N side in groups of 8: a decoding tile of 4 or 8 rows fills it where it would leave half or more of the
+// M side empty. A 16-byte load from a block in shared memory holds the codes of a thread's own operand registers (the contraction
+// index of a product may be dealt in any order as long as both operands agree). They become fp16 by one conversion and one
+// product with the block's scale, both exact; the row's power of two goes into the score, or into the weight:
+//   keys     s = 2^e_k (code scale . q) / sqrt(d); the query row is held in fp16 times a power of two that brings its largest entry to
+//            2^14, so bf16 entries down to 2^-31 of that are exact
+//   values   w = e^(s - max) 2^(e_v - E) 2^14 in fp16 (11 bits; the sum of the weights is of the unrounded ones), E the largest exponent of the
+//            values so far: like the running maximum, the accumulators follow it when it grows
+// A transposed 8x8 register exchange (movmatrix) turns P into the second product's operand: nothing goes through shared memory but the blocks.
+//
+// A warp takes every fourth block of its CTA's keys, in a ring of its own filled by bulk copies (one per block): warps never wait for one
+// another until the end. A tile's keys are cut over a cluster of CTAs when there are few tiles; the parts are joined through distributed shared
+// memory in a fixed order, so there is one launch, no scratch memory, and the same bits in every call.
+constexpr int A4_WARPS = 4, A4_STAGES = 2, A4_MAX_CLUSTER = 16, A4_ROWS_MAX = 16;
+constexpr int A4_BIAS = 14;            // weights are kept times 2^14
+
+struct A4Shared {
+  uint64_t full[A4_WARPS][A4_STAGES];
+  float max_[A4_WARPS][A4_ROWS_MAX], den[A4_WARPS][A4_ROWS_MAX];         // per warp and row
+  float row_max[A4_ROWS_MAX], row_den[A4_ROWS_MAX];                      // of the CTA
+  uint32_t abort_flag;
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four bytes of two e2m1 codes each -> four pairs of fp16.
+__device__ __forceinline__ void e2m1_pairs(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 x, y, z, w;\n\t"
+      "mov.b32 {x, y, z, w}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, x;\n\tcvt.rn.f16x2.e2m1x2 %1, y;\n\tcvt.rn.f16x2.e2m1x2 %2, z;\n\tcvt.rn.f16x2.e2m1x2 %3, w;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+// The two e4m3 scales in the low half of w -> a pair of fp16.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float a4_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t* p) {
+  static_assert(N == 2 || N == 4, "8 or 16 bytes");
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+}
+// 2^14 over the power of two of a row's largest magnitude, and back.
+__device__ __forceinline__ int a4_query_exponent(float most) {
+  return most > 0.0f && most < INFINITY ? min(max((__float_as_int(most) >> 23) - 127, -100), 127) : 0;
+}
+
+template <int K, int V>
+__host__ __device__ constexpr int a4_block_bytes() { return 36 * (K + V) + 2 * C4_TOKENS; }
+// The warps' rings; at the end the same memory holds the warps' outputs, rows of V floats.
+template <int K, int V, int NT>
+__host__ __device__ constexpr int a4_ring_bytes() {
+  const int ring = A4_WARPS * A4_STAGES * a4_block_bytes<K, V>(), out = (A4_WARPS + 1) * 8 * NT * V * 4;
+  return ring > out ? ring : out;
+}
+
+template <int K, int V, int NT>
+__global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_kernel(const PagedAttn a, const Cache4 c) {
+  constexpr int BYTES = a4_block_bytes<K, V>(), KS = K / 16, KW = K / 32, ROWS = 8 * NT;
+  extern __shared__ __align__(128) uint8_t a4_raw[];
+  uint8_t* ring_all = a4_raw;
+  A4Shared* sh = reinterpret_cast<A4Shared*>(a4_raw + a4_ring_bytes<K, V, NT>());
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  uint32_t rank, ctas;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < A4_WARPS; ++w)
+      for (int s = 0; s < A4_STAGES; ++s) mbar_init(&sh->full[w][s], 1);
+    sh->abort_flag = *reinterpret_cast<volatile int*>(&g_wait_timeouts) != 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  launch_next();
+  wait_previous();
+
+  // ---- the tile ----
+  const int tile = blockIdx.x / ctas, group = blockIdx.y;
+  int tok0, ntok;
+  i64 seq;
+  if (a.tiles) {
+    const int* t = a.tiles + (i64)tile * 3;
+    seq = t[0], tok0 = t[1], ntok = t[2];
+  } else {
+    tok0 = tile, ntok = 1;
+    seq = a.seq[tok0];
+  }
+  const int row0 = blockIdx.z * ROWS, rows = min(ROWS, ntok * a.H - row0);
+  if (rows <= 0) return;                                   // all CTAs of the cluster alike
+  const i64 limit = (i64)a.nblk * a.bs - 1;
+  const int t_first = row0 / a.H, t_last = (row0 + rows - 1) / a.H;
+  const i64 p_first = min(a.pos[tok0 + t_first], limit), p_last = min(a.pos[tok0 + t_last], limit);
+  const int lo_all = a.first_key(p_first), b_lo = lo_all / C4_TOKENS, b_hi = p_last < 0 ? b_lo : (int)(p_last / C4_TOKENS) + 1;
+  const int b0 = b_lo + (int)((i64)(b_hi - b_lo) * rank / ctas), b1 = b_lo + (int)((i64)(b_hi - b_lo) * (rank + 1) / ctas);
+  const int n = b1 - b0 > warp ? (b1 - b0 - warp + A4_WARPS - 1) / A4_WARPS : 0;          // the warp's blocks: b0 + warp + 4 i
+  uint8_t* ring = ring_all + warp * A4_STAGES * BYTES;
+  bool ok = sh->abort_flag == 0;
+
+  int held = 0;
+  auto fetch = [&](int i) {                                // block i of the warp; the warp reads the block table for 32 blocks at a time
+    if ((i & 31) == 0) {
+      const int b = min(b0 + warp + (i + lane) * A4_WARPS, b_hi - 1);
+      held = (int)a.page_of(seq, min(b * C4_TOKENS / a.bs, a.nblk - 1));
+    }
+    const i64 page = __shfl_sync(0xffffffffu, held, i & 31);
+    if (lane == 0) {
+      const int in_page = (b0 + warp + i * A4_WARPS) % (a.bs / C4_TOKENS);
+      uint64_t* bar = &sh->full[warp][i % A4_STAGES];
+      mbar_arrive_expect_tx(bar, BYTES);
+      bulk_load(ring + i % A4_STAGES * BYTES, c.p + ((page * a.G + group) * (a.bs / C4_TOKENS) + in_page) * BYTES, bar, BYTES);
+    }
+  };
+  if (ok)
+    for (int i = 0; i < A4_STAGES && i < n; ++i) fetch(i);
+
+  // ---- queries: thread (gid, tig) holds, of row gid of every group of 8, entries tig K / 4 .. ----
+  uint32_t q[NT][KS][2];
+  float row_scale[NT][2];                                  // of rows 2 tig, 2 tig + 1: what a score is worth in powers of two
+  int row_lo[NT][2], row_hi[NT][2];
+  const bool wide = a.ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int flat = row0 + min(8 * t + gid, rows - 1);
+    const bf16* from = static_cast<const bf16*>(a.q) + (((i64)group * a.M + tok0 + flat / a.H) * a.H + flat % a.H) * a.ldq + tig * (K / 4);
+    float most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d = tig * (K / 4) + 4 * s;
+      if (wide && d + 4 <= a.W) {
+        const uint2 v = *reinterpret_cast<const uint2*>(from + 4 * s);
+        q[t][s][0] = v.x, q[t][s][1] = v.y;
+      } else {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = d + e < a.W ? ld(from + 4 * s + e) : 0.0f;
+        q[t][s][0] = pack_bf16(v[0], v[1]);
+        q[t][s][1] = pack_bf16(v[2], v[3]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(q[t][s][h] << 16)), fabsf(__uint_as_float(q[t][s][h] & 0xffff0000u))));
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const int e = a4_query_exponent(most);
+    // times 2^(14 - e), in two steps that cannot overflow on their own
+    const float up = c4_power((A4_BIAS - e) / 2), up2 = c4_power(A4_BIAS - e - (A4_BIAS - e) / 2);
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        q[t][s][h] = pack_half(__uint_as_float(q[t][s][h] << 16) * up * up2, __uint_as_float(q[t][s][h] & 0xffff0000u) * up * up2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int back = __shfl_sync(0xffffffffu, e, (2 * tig + h) * 4) - A4_BIAS;
+      row_scale[t][h] = a.scale * 1.4426950408889634f * c4_power(back / 2) * c4_power(back - back / 2);
+      const int f = row0 + min(8 * t + 2 * tig + h, rows - 1);
+      const i64 p = min(a.pos[tok0 + f / a.H], limit);
+      row_lo[t][h] = a.first_key(p);
+      row_hi[t][h] = (int)p;
+    }
+  }
+  const int whole_lo = a.first_key(p_last), whole_hi = (int)p_first;       // keys that every row sees
+
+  float out[V / 16][NT][4] = {};                           // entries 16 j + gid (+ 8) of rows 2 tig (+ 1)
+  float top[NT][2], den[NT][2];
+  int E = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) top[t][h] = -INFINITY, den[t][h] = 0.0f;
+
+  for (int i = 0; ok && i < n; ++i) {
+    if (!mbar_wait(&sh->full[warp][i % A4_STAGES], (i / A4_STAGES) & 1)) ok = false;
+    if (!__all_sync(0xffffffffu, ok)) {
+      // give up: what is in flight has to land before the memory is used for anything else
+      ok = false;
+      if (lane == 0) {
+        atomicAdd(&g_wait_timeouts, 1);
+        for (int k = i; k < min(n, i + A4_STAGES); ++k) mbar_wait(&sh->full[warp][k % A4_STAGES], (k / A4_STAGES) & 1);
+      }
+      __syncwarp();
+      break;
+    }
+    const uint8_t* blk = ring + i % A4_STAGES * BYTES;
+    const int k0 = (b0 + warp + i * A4_WARPS) * C4_TOKENS;
+
+    // ---- scores: m-tile u holds tokens 16 (gid / 2) + 4 u + gid % 2 in its rows gid, and those + 2 in rows gid + 8 ----
+    float s[4][NT][4] = {};
+    const int tok = (gid >> 1) * 16 + (gid & 1);
+    uint32_t ks[K / 32];
+    lds<K / 32>(ks, blk + 32 * K + (((gid >> 1) * 2 + (gid & 1)) * (K / 16) + tig * (K / 64)) * 8);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t k_lo[KW], k_hi[KW];
+      lds<KW>(k_lo, blk + (tok + 4 * u) * (K / 2) + tig * (K / 8));
+      lds<KW>(k_hi, blk + (tok + 4 * u + 2) * (K / 2) + tig * (K / 8));
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {                       // 8 codes: two steps of the contraction, within a block of 16
+        const int j = w / 2;
+        uint32_t lo[4], hi[4];
+        const uint32_t pair = e4m3_pair(ks[j * 2 + u / 2] >> (u % 2 * 16));
+        const uint32_t s_lo = __byte_perm(pair, 0, 0x1010), s_hi = __byte_perm(pair, 0, 0x3232);
+        e2m1_pairs(k_lo[w], lo);
+        e2m1_pairs(k_hi[w], hi);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) lo[x] = hmul2(lo[x], s_lo), hi[x] = hmul2(hi[x], s_hi);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          mma_f16(s[u][t], lo[0], hi[0], lo[1], hi[1], q[t][2 * w][0], q[t][2 * w][1]);
+          mma_f16(s[u][t], lo[2], hi[2], lo[3], hi[3], q[t][2 * w + 1][0], q[t][2 * w + 1][1]);
+        }
+      }
+    }
+
+    // ---- exponents of the thread's tokens tok + 2 x, x = 0 .. 7: bytes 0 and 2 of four words ----
+    uint32_t ke[4], ve[4];
+    lds<4>(ke, blk + 36 * (K + V) + (gid >> 1) * 16);
+    lds<4>(ve, blk + 36 * (K + V) + C4_TOKENS + (gid >> 1) * 16);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      ke[w] = ke[w] >> ((gid & 1) * 8) & 0x00ff00ffu;
+      ve[w] = ve[w] >> ((gid & 1) * 8) & 0x00ff00ffu;
+    }
+    const bool edge = k0 < whole_lo || k0 + C4_TOKENS - 1 > whole_hi;
+    if (edge) {                                            // exponents of tokens that no row of the tile sees
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int key = k0 + tok + 2 * x;
+        if (key < lo_all || key > p_last) ve[x / 2] &= x % 2 ? 0x000000ffu : 0x00ff0000u;
+      }
+    }
+    uint32_t big = __vmaxu2(__vmaxu2(ve[0], ve[1]), __vmaxu2(ve[2], ve[3]));
+    int e_new = max(E, (int)max(big & 0xffffu, big >> 16));
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, o));
+
+    // ---- the running maximum ----
+    bool grows = e_new > E;
+    const float f_e = E == 0 ? 0.0f : c4_power(max(E - e_new, -126));
+    float f[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {                    // key rows gid and gid + 8 of m-tile u: token tok + 2 (2 u + x)
+            float& v = s[u][t][2 * x + h];
+            v *= __uint_as_float(x ? ke[u] << 7 & 0x7f800000u : ke[u] << 23) * row_scale[t][h];
+            if (edge) {
+              const int key = k0 + tok + 4 * u + 2 * x;
+              if (key < row_lo[t][h] || key > row_hi[t][h]) v = -INFINITY;
+            }
+            m = fmaxf(m, v);
+          }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        f[t][h] = f_e;
+        if (m > top[t][h]) {
+          const float g = a4_exp2(top[t][h] - m);          // 0 for the first keys
+          f[t][h] *= g;
+          den[t][h] *= g;
+          top[t][h] = m;
+          grows = true;
+        }
+      }
+    E = e_new;
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int j = 0; j < V / 16; ++j)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) out[j][t][x] *= f[t][x & 1];
+    }
+
+    // ---- weights: their sum as they are, then times the values' powers of two, transposed ----
+    uint32_t p[4][NT][2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float g[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int e = (int)(x ? ve[u] >> 16 : ve[u] & 0xffffu) - E + 127 + A4_BIAS;
+        g[x] = __int_as_float(max(e, 0) << 23);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float w[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float m = top[t][h] == -INFINITY ? 0.0f : top[t][h];
+            w[h] = a4_exp2(s[u][t][2 * x + h] - m);
+            den[t][h] += w[h];
+            w[h] *= g[x];
+          }
+          p[u][t][x] = transposed(pack_half(w[0], w[1]));
+        }
+    }
+
+    // ---- values: entries 16 j + gid and + 8 of tokens 16 tig .. + 15 ----
+#pragma unroll
+    for (int j = 0; j < V / 16; ++j) {
+      uint32_t vc[4], vs[4];
+      lds<4>(vc, blk + 36 * K + (j * 8 + gid) * C4_TOKENS + tig * 16);
+      lds<4>(vs, blk + 36 * K + 32 * V + j * C4_TOKENS + tig * 16);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t x[4];
+        e2m1_pairs(vc[u], x);
+        const uint32_t s01 = e4m3_pair(vs[u]), s23 = e4m3_pair(vs[u] >> 16);
+        const uint32_t a0 = hmul2(__byte_perm(x[0], x[1], 0x5410), s01), a1 = hmul2(__byte_perm(x[0], x[1], 0x7632), s01);
+        const uint32_t a2 = hmul2(__byte_perm(x[2], x[3], 0x5410), s23), a3 = hmul2(__byte_perm(x[2], x[3], 0x7632), s23);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) mma_f16(out[j][t], a0, a1, a2, a3, p[u][t][0], p[u][t][1]);
+      }
+    }
+    __syncwarp();                                          // the block is read: its place may be filled again
+    if (i + A4_STAGES < n) fetch(i + A4_STAGES);
+  }
+
+  // ---- the CTA's part: rows of V outputs per warp, in units of 1 ----
+  if (!ok) sh->abort_flag = 1;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) den[t][h] += __shfl_xor_sync(0xffffffffu, den[t][h], o);
+      if (gid == 0) sh->max_[warp][8 * t + 2 * tig + h] = top[t][h], sh->den[warp][8 * t + 2 * tig + h] = den[t][h];
+    }
+  __syncthreads();                                         // all rings are done with
+  const bool dead = sh->abort_flag != 0;
+  float* slab = reinterpret_cast<float*>(ring_all);        // [row][V] of the CTA, then of every warp
+  const float unit = E == 0 ? 0.0f : c4_power(max(E - 127 - A4_BIAS, -126));
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * t + 2 * tig + h;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < A4_WARPS; ++w) m = fmaxf(m, sh->max_[w][r]);
+      const float g = unit * (top[t][h] == -INFINITY ? 0.0f : a4_exp2(top[t][h] - m));
+#pragma unroll
+      for (int j = 0; j < V / 16; ++j) {
+        slab[((warp + 1) * ROWS + r) * V + 16 * j + gid] = out[j][t][h] * g;
+        slab[((warp + 1) * ROWS + r) * V + 16 * j + gid + 8] = out[j][t][h + 2] * g;
+      }
+      if (warp == 0 && gid == 0) {
+        float d = 0.0f;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w) d += sh->max_[w][r] == -INFINITY ? sh->den[w][r] : sh->den[w][r] * a4_exp2(sh->max_[w][r] - m);
+        sh->row_max[r] = m;
+        sh->row_den[r] = d;
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * V; i += 32 * A4_WARPS) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 1; w <= A4_WARPS; ++w) v += slab[w * ROWS * V + i];
+    slab[i] = v;
+  }
+  cluster_arrive();
+  cluster_wait();
+  // ---- the row: every CTA of the cluster finishes a part of the outputs ----
+  if (!dead) {
+    const uint32_t slab_at = smem_u32(slab), max_at = smem_u32(sh->row_max), den_at = smem_u32(sh->row_den);
+    for (int i = rank * 32 * A4_WARPS + threadIdx.x; i < rows * V; i += ctas * 32 * A4_WARPS) {
+      const int r = i / V, d = i % V, flat = row0 + r, head = group * a.H + flat % a.H;
+      if (d >= a.R) continue;
+      float m = a.sink ? a.sink[head] * 1.4426950408889634f : -INFINITY, sum = 0.0f, v = 0.0f;
+      const float sink = m;
+      for (uint32_t k = 0; k < ctas; ++k) m = fmaxf(m, ld_cluster(mapa_shared(max_at + 4 * r, k)));
+      if (a.sink) sum = a4_exp2(sink - m);
+      for (uint32_t k = 0; k < ctas; ++k) {
+        const float mk = ld_cluster(mapa_shared(max_at + 4 * r, k)), dk = ld_cluster(mapa_shared(den_at + 4 * r, k));
+        const float g = mk == -INFINITY ? (dk == 0.0f ? 0.0f : 1.0f) : a4_exp2(mk - m);      // a part with no key has no weight
+        sum += g * dk;
+        v += g * ld_cluster(mapa_shared(slab_at + 4 * i, k));
+      }
+      st(static_cast<bf16*>(a.out) + (tok0 + flat / a.H) * a.out_tok + head * a.out_head + d, sum == 0.0f ? 0.0f : v / sum);
+    }
+  }
+  cluster_arrive();                                        // nobody leaves while its memory may be read
+  cluster_wait();
 }
 
 }  // namespace bxf

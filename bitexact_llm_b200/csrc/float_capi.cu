@@ -312,9 +312,43 @@ int launch_store4(const Store4<T>& a, cudaStream_t st) {
   return launch_chained(fl_store4_kernel<T, 32>, dim3(ceil_div(a.M, 32), a.c.G), S4_THREADS, (a.c.V / 2 + a.c.V / 16 + 1) * 36, st, 0, a);
 }
 
-template <class T>
-int launch_attention4(const PagedAttn& a, const Cache4& c, int variant, cudaStream_t st) {
-  return launch_chained(fl_attention4_plain_kernel<T>, dim3(a.M, a.H * a.G), A4_THREADS, (c.K + 2 * c.V) * 4, st, 0, a, c);
+bool attention4_fits(int dtype, const Cache4& c) { return dtype == BXF_BF16 && c.K <= 128 && c.V <= 128; }
+
+// CTAs that share the keys of a tile: a power of two, until the SMs have their three CTAs, as long as every warp has a block to work on.
+int attention4_cluster(i64 tiles, i64 blocks, int per_sm) {
+  int c = 1;
+  while (c < A4_MAX_CLUSTER && tiles * c * 2 <= (i64)per_sm * device_sms() && blocks >= 2 * c * A4_WARPS) c *= 2;
+  return c;
+}
+
+template <int K, int V, int NT>
+int launch_attention4(const PagedAttn& a, const Cache4& c, cudaStream_t st) {
+  constexpr int smem = a4_ring_bytes<K, V, NT>() + sizeof(A4Shared), per_sm = NT == 1 ? 3 : 2;
+  static PerDevice configured;
+  if (once_per_device(configured, [] {
+        const cudaError_t e = cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      }) != BX_OK)
+    return BX_ELAUNCH;
+  const int n = a.tiles ? a.ntiles : a.M, rows = a.tiles ? (a.H > 128 ? a.H : 128) : a.H, z = ceil_div(rows, 8 * NT);
+  const int cluster = attention4_cluster((i64)n * a.G * z, (i64)a.nblk * a.bs / C4_TOKENS, per_sm);
+  return launch_chained(fl_attention4_kernel<K, V, NT>, dim3((unsigned)n * cluster, a.G, z), 32 * A4_WARPS, smem, st, cluster, a, c);
+}
+
+template <int NT>
+int launch_attention4(const PagedAttn& a, const Cache4& c, cudaStream_t st) {
+  if (c.K == 64) return c.V == 64 ? launch_attention4<64, 64, NT>(a, c, st) : launch_attention4<64, 128, NT>(a, c, st);
+  return c.V == 64 ? launch_attention4<128, 64, NT>(a, c, st) : launch_attention4<128, 128, NT>(a, c, st);
+}
+
+int run_attention4(int dtype, const PagedAttn& a, const Cache4& c, int variant, cudaStream_t st) {
+  const bool fits = attention4_fits(dtype, c) && (!a.tiles || a.ntiles > 0) && a.G <= 65535;
+  if (variant == 2 && !fits) return BX_ELIMIT;
+  if (variant != 1 && fits) return a.tiles || a.H > 8 ? launch_attention4<2>(a, c, st) : launch_attention4<1>(a, c, st);
+  const dim3 grid(a.M, a.H * a.G);
+  const int smem = (c.K + 2 * c.V) * 4;
+  if (dtype == BXF_F32) return launch_chained(fl_attention4_plain_kernel<float>, grid, A4_THREADS, smem, st, 0, a, c);
+  return launch_chained(fl_attention4_plain_kernel<bf16>, grid, A4_THREADS, smem, st, 0, a, c);
 }
 
 bool gru_ok(const bxf_gru* g, int M, int width) {
@@ -701,7 +735,7 @@ int bxf_gqa_attention4(int dtype, const void* q, int64_t ldq, int M, int heads, 
   const Cache4 c = cache4_of(cache, kv_heads, dim, vdim, page, nb);
   const PagedAttn a{q, ldq, M, heads / kv_heads, kv_heads, dim, vdim, 0, cache, c.bytes(), page, nb, bt, bt_is64, bt_stride, nblk,
                     reinterpret_cast<const i64*>(seq), reinterpret_cast<const i64*>(pos), tiles, ntiles, window, sink, scale, out, ldo, vdim};
-  return dtype == BXF_F32 ? launch_attention4<float>(a, c, variant, stream_of(stream)) : launch_attention4<bf16>(a, c, variant, stream_of(stream));
+  return run_attention4(dtype, a, c, variant, stream_of(stream));
 }
 
 int bxf_streams(int dtype, const bxf_streams_step* p, int M, void* stream) {
