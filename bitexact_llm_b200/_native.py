@@ -230,17 +230,21 @@ def ptr(t):
 
 
 def stream():
+    """The current stream of the current device, as a number."""
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def here(*tensors):
     """Refuses tensors of the host, or of another device than the current one, whose stream the kernels go to."""
     import torch
-    dev = torch.cuda.current_device()
+    dev = -1
     for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+        if t is not None:
+            if dev < 0 and t.is_cuda:
+                dev = torch._C._cuda_getDevice()
+            if dev < 0 or t.get_device() != dev:
+                raise ValueError(f"a tensor is on {t.device}, not on the current CUDA device")
 
 
 def device_status():

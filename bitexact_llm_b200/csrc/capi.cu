@@ -448,11 +448,19 @@ int exact_linear_auto(int M, int N, int K, bool residual) {
   return 100 * cost[best] < 99 * given ? forms[best] : form;
 }
 
-// CTAs that share a row: as many as fill the SMs several times over while a CTA still reads 32 KB.
-int log_probs_cluster(int M, int V, int bytes) {
-  int c = 1;
-  while (c < LP_MAX_CLUSTER && (long long)M * c < 4ll * 4 * device_sms() && (long long)V * bytes / (2 * c) >= 32768) c *= 2;
-  return c;
+// CTAs that share a row: the power of two with the least estimated time, rounds of the resident CTAs (four to an SM) times a CTA's
+// part of the row at its share of the memory's rate and what a CTA costs beside it (us, measured as the slope over many small
+// parts: joining 4, with the best list 9).
+int log_probs_cluster(int M, int V, int bytes, bool top) {
+  const long long resident = 4ll * device_sms();
+  const double row = (double)V * bytes / (6.0e6 / resident), own = top ? 9.0 : 4.0;
+  int best = 1;
+  double least = 0.0;
+  for (int c = 1; c <= LP_MAX_CLUSTER; c *= 2) {
+    const double t = (double)((M * (long long)c + resident - 1) / resident) * (row / c + own);
+    if (c == 1 || t < least) least = t, best = c;
+  }
+  return best;
 }
 
 template <class T, bool TOP>
@@ -462,7 +470,7 @@ int launch_log_probs(const LogProbs& a, int M, cudaStream_t st) {
         return cudaFuncSetAttribute(log_probs_kernel<T, TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       }) != BX_OK)
     return BX_ELAUNCH;
-  const int c = log_probs_cluster(M, a.V, sizeof(T));
+  const int c = log_probs_cluster(M, a.V, sizeof(T), TOP);
   return launch_chained(log_probs_kernel<T, TOP>, dim3((unsigned)M * c), LP_THREADS, sizeof(LpShared<typename LpOf<T>::Val>), st, c, a);
 }
 
@@ -1828,7 +1836,7 @@ int bx_log_probs(int kind, const void* logits, int64_t ld, const int64_t* tok, i
   if (!logits || !entropy || (tok && (!logp || !rank)) || (top && (!top_ids || !top_logp)) || !aligned_to(logits, kind == BX_LOGITS_I64 ? 8 : kind == BX_LOGITS_F32 ? 4 : 2))
     return BX_EARG;
   const int shift = fr > 24 ? fr - 24 : 0;
-  const LogProbs a{logits, ld, reinterpret_cast<const long long*>(tok), V, top, shift, 1.0f / (float)(1ll << (fr - shift)), logp, entropy,
+  const LogProbs a{logits, ld, reinterpret_cast<const long long*>(tok), V, top, shift, fr >= 8 && shift == 0, 1.0f / (float)(1ll << (fr - shift)), logp, entropy,
                    reinterpret_cast<long long*>(rank), reinterpret_cast<long long*>(top_ids), top_logp};
   cudaStream_t st = (cudaStream_t)stream;
   if (kind == BX_LOGITS_I64) return top ? launch_log_probs<long long, true>(a, M, st) : launch_log_probs<long long, false>(a, M, st);

@@ -66,48 +66,78 @@ __device__ __forceinline__ int c4_scale_for(float most) {
   c += 6.0f * c4_scale(c) < most;
   return c;
 }
-// The nearest code of x in steps of `step`: x is held against exact multiples of it.
-__device__ __forceinline__ int c4_nearest(float x, float step) {
-  const float m = fabsf(x);
-  int c = (m > 0.25f * step) + (m >= 0.75f * step) + (m > 1.25f * step) + (m >= 1.75f * step) + (m > 2.5f * step) + (m >= 3.5f * step) +
-          (m > 5.0f * step);
-  if (step == 0.0f) c = 0;
-  return x < 0.0f ? c | 8 : c;
+// Codes of four entries in steps of `step` (inv = 1 / step rounded; both 0 where the block is): the quotient, corrected by its exact
+// remainder, is the correctly rounded one, and exact where it is a tie. The entries of bf16 rows come no nearer to a tie without being
+// one than 2^-12 of it; those of 32-bit rows may round to one, and are set beside it by the sign of what remains.
+template <class T>
+__device__ __forceinline__ int c4_codes(const float (&y)[4], float step, float inv) {
+  float q[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float t = y[k] * inv;
+    q[k] = fmaf(fmaf(-t, step, y[k]), inv, t);
+    if constexpr (sizeof(T) == 4) {
+      const float rest = fmaf(-q[k], step, y[k]);
+      const int bits = __float_as_int(q[k]), outward = (rest > 0.0f) == (q[k] > 0.0f) ? 1 : -1;
+      if (rest != 0.0f && q[k] != 0.0f) q[k] = __int_as_float(bits + outward);
+    }
+  }
+  uint32_t c;
+  asm("{\n\t.reg .b8 x, y, z;\n\tmov.b32 {x, y, z, _}, 0;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 x, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 y, %4, %3;\n\tmov.b32 %0, {x, y, z, z};\n\t}"
+      : "=r"(c)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+  return (int)c;
 }
 
-// A warp's row: lane l holds entries 128 i + 4 l .. + 3.
+// A warp's row: lane l holds entries 128 i + 4 l .. + 3, i < N.
+template <class T, int N>
 struct C4Row {
-  float x[C4_MAX / 128][4];
-  bool bad;                            // of the lane's entries
+  float x[N][4];
 
-  template <class T>
-  __device__ __forceinline__ float load(const T* p, int n, int lane) {           // -> the largest finite magnitude of the row
-    float most = 0.0f;
-    bad = false;
+  __device__ __forceinline__ void load(const T* p, int n, int lane) {
+    const bool wide = (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll
-    for (int i = 0; i < C4_MAX / 128; ++i)
+    for (int i = 0; i < N; ++i) {
+      const int d = 128 * i + 4 * lane;
+      if (wide && d + 4 <= n) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p + d);
+          x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(p + d);
+          x[i][0] = __uint_as_float(v.x << 16), x[i][1] = __uint_as_float(v.x & 0xffff0000u);
+          x[i][2] = __uint_as_float(v.y << 16), x[i][3] = __uint_as_float(v.y & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[i][k] = d + k < n ? ld(p + d + k) : 0.0f;
+      }
+    }
+  }
+  // -> the largest finite magnitude of the row; whether all of the lane's entries are finite. Those that are not become 0.
+  __device__ __forceinline__ float most(bool& fine) {
+    float m = 0.0f;
+    fine = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int d = 128 * i + 4 * lane + k;
-        float v = d < n ? ld(p + d) : 0.0f;
-        if (!(fabsf(v) < INFINITY)) bad = true, v = 0.0f;
-        x[i][k] = fminf(fmaxf(v, -1.7014118e38f), 1.7014118e38f);
-        most = fmaxf(most, fabsf(x[i][k]));
+        if (!(fabsf(x[i][k]) < INFINITY)) fine = false, x[i][k] = 0.0f;
+        x[i][k] = fminf(fmaxf(x[i][k], -1.7014118e38f), 1.7014118e38f);
+        m = fmaxf(m, fabsf(x[i][k]));
       }
-    return warp_max(most);
+    return warp_max(m);
   }
   // Codes of the lane's four entries (4 bits each) and the scale of their block.
   __device__ __forceinline__ int codes(int i, float unit, int& scale) const {
     const float y[4] = {x[i][0] * unit, x[i][1] * unit, x[i][2] * unit, x[i][3] * unit};
-    float most = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    scale = c4_scale_for(most);
+    float m = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    scale = c4_scale_for(m);
     const float step = c4_scale(scale);
-    int c = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) c |= c4_nearest(y[k], step) << (4 * k);
-    return c;
+    return c4_codes<T>(y, step, step > 0.0f ? __frcp_rn(step) : 0.0f);
   }
 };
 
@@ -129,7 +159,7 @@ constexpr int S4_THREADS = 128;
 
 // ROWS rows of one head per CTA, a warp per row. Keys go out as they are made (a row is contiguous); the bytes of values lie along the
 // tokens: with many rows they are put together in shared memory, and 16 (or 4) rows that lie in a run of slots go out as one store.
-template <class T, int ROWS>
+template <class T, int ROWS, int N>
 __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a) {
   constexpr int PITCH = ROWS + 4;      // bytes of a value column of the CTA's rows
   extern __shared__ __align__(16) uint8_t s4_smem[];
@@ -145,18 +175,27 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
   }
   __syncthreads();
   const int columns = c.V / 2 + c.V / 16 + 1;              // of value bytes: codes, scales, the exponent
+  C4Row<T, N> k, v, k_next, v_next;
+  auto fetch = [&](int r) {
+    if (r >= ROWS || slots[r] < 0) return;
+    const i64 m = row0 + r;
+    k_next.load(a.k + m * a.k_row + g * a.k_head, c.dim, lane);
+    v_next.load(a.v + m * a.v_row + g * a.v_head, c.vdim, lane);
+  };
+  fetch(warp);
   for (int r = warp; r < ROWS; r += S4_THREADS / 32) {
+    k = k_next, v = v_next;
+    fetch(r + S4_THREADS / 32);
     if (slots[r] < 0) continue;
-    const int m = row0 + r, tok = (int)(slots[r] % C4_TOKENS);
+    const int tok = (int)(slots[r] % C4_TOKENS);
     uint8_t* block = c.block(slots[r], g);
-    C4Row k, v;
-    const float most_k = k.load(a.k + m * a.k_row + g * a.k_head, c.dim, lane);
-    const float most_v = v.load(a.v + m * a.v_row + g * a.v_head, c.vdim, lane);
-    const bool bad = __any_sync(0xffffffffu, k.bad || v.bad);
+    bool fine_k, fine_v;
+    const float most_k = k.most(fine_k), most_v = v.most(fine_v);
+    const bool bad = !__all_sync(0xffffffffu, fine_k && fine_v);
     const int ek = c4_exponent(most_k), ev = c4_exponent(most_v);
     const float uk = c4_power(-ek), uv = bad ? 0.0f : c4_power(-ev);
 #pragma unroll
-    for (int i = 0; i < C4_MAX / 128; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (128 * i >= c.K) break;
       int scale;
       const int code = k.codes(i, uk, scale), d = 128 * i + 4 * lane;
@@ -166,7 +205,7 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
       }
     }
 #pragma unroll
-    for (int i = 0; i < C4_MAX / 128; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (128 * i >= c.V) break;
       int scale;
       const int code = v.codes(i, uv, scale), other = __shfl_xor_sync(0xffffffffu, code, 2), d = 128 * i + 4 * lane;
@@ -220,24 +259,46 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
   }
 }
 
-// The entries that the cache holds at `slot`: k T [M][G][dim], v T [M][G][vdim]; slots outside the cache give zeros. A CTA per row and head.
+// The entries that the cache holds at `slot`: k T [M][G][dim], v T [M][G][vdim]; slots outside the cache give zeros. A warp per row and
+// head, a lane for four entries (the codes of a key row lie together; a lane's four of a value are four bytes 64 apart).
+constexpr int R4_WARPS = 8;
+
 template <class T>
-__global__ void __launch_bounds__(128) fl_read4_kernel(const Cache4 c, const i64* slot, T* k, T* v, int M) {
+__device__ __forceinline__ void c4_put(T* p, int d, int n, const float (&x)[4]) {
+  if (d + 4 <= n && (reinterpret_cast<uintptr_t>(p + d) & (4 * sizeof(T) - 1)) == 0) st4(p + d, x[0], x[1], x[2], x[3]);
+  else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (d + q < n) st(p + d + q, x[q]);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(32 * R4_WARPS) fl_read4_kernel(const Cache4 c, const i64* slot, T* k, T* v, i64 rows) {
   launch_next();
   wait_previous();
-  const int m = blockIdx.x, g = blockIdx.y;
-  const i64 s = slot[m], at = (i64)m * c.G + g;
+  const i64 at = (i64)blockIdx.x * R4_WARPS + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (at >= rows) return;
+  const i64 s = slot[at / c.G];
   const bool in = s >= 0 && s < (i64)c.nb * c.page;
   const int tok = in ? (int)(s % C4_TOKENS) : 0;
-  const uint8_t* b = c.block(in ? s : 0, g);
-  const float pk = __int_as_float(b[c.key_exp(tok)] << 23), pv = __int_as_float(b[c.value_exp(tok)] << 23);
-  for (int d = threadIdx.x; d < c.dim; d += 128) {
-    const float x = c4_code(b[tok * (c.K / 2) + d / 2] >> (d % 2 * 4) & 15) * c4_scale(b[c.key_scale(tok, d / 16)] & 127) * pk;
-    st(k + at * c.dim + d, in ? x : 0.0f);
+  const uint8_t* b = c.block(in ? s : 0, (int)(at % c.G));
+  const float pk = in ? __int_as_float(b[c.key_exp(tok)] << 23) : 0.0f, pv = in ? __int_as_float(b[c.value_exp(tok)] << 23) : 0.0f;
+  for (int d = 4 * lane; d < c.dim; d += 128) {
+    const int w = *reinterpret_cast<const uint16_t*>(b + tok * (c.K / 2) + d / 2);
+    const float f = c4_scale(b[c.key_scale(tok, d / 16)] & 127);
+    float x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = in ? c4_code(w >> (4 * q) & 15) * f * pk : 0.0f;
+    c4_put(k + at * c.dim, d, c.dim, x);
   }
-  for (int d = threadIdx.x; d < c.vdim; d += 128) {
-    const float x = c4_code(b[c.value_code(tok, d / 16, d % 8)] >> (d % 16 / 8 * 4) & 15) * c4_scale(b[c.value_scale(tok, d / 16)] & 127) * pv;
-    st(v + at * c.vdim + d, in ? x : 0.0f);
+  for (int d = 4 * lane; d < c.vdim; d += 128) {
+    const float f = c4_scale(b[c.value_scale(tok, d / 16)] & 127);
+    float x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = in ? c4_code(b[c.value_code(tok, d / 16, d % 8 + q)] >> (d % 16 / 8 * 4) & 15) * f * pv : 0.0f;
+    c4_put(v + at * c.vdim, d, c.vdim, x);
   }
 }
 

@@ -39,7 +39,30 @@ __device__ __forceinline__ int st_owner(const int* ends, int n, int i) {
   return lo;
 }
 
-__device__ __forceinline__ int st_pages(long long n, int page) { return (int)((n + page - 1) / page); }
+__device__ __forceinline__ int st_pages(int n, int page) { return (int)(((unsigned)n + page - 1) / (unsigned)page); }
+
+// Inclusive sums over a warp.
+__device__ __forceinline__ void st_scan(long long& r, int& p, int& t, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long r2 = __shfl_up_sync(0xffffffffu, r, o);
+    const int p2 = __shfl_up_sync(0xffffffffu, p, o), t2 = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) r += r2, p += p2, t += t2;
+  }
+}
+
+// Row i, of request b (-1: padding). `full`: pages on the stack before any were taken.
+__device__ __forceinline__ void st_row(const StepTables& a, int i, int b, const int* row_end, const int* take_end, const int* base, int full) {
+  if (b < 0) {
+    a.seq[i] = 0, a.pos[i] = 0, a.slot[i] = -1;
+    return;
+  }
+  const int start = base[b], pos = start + i - (b ? row_end[b - 1] : 0);
+  const int held = st_pages(start, a.page), block = (int)((unsigned)pos / (unsigned)a.page);
+  const int page = block < held ? a.bt[b * a.bt_stride + block]
+                                : *const_cast<volatile int*>(a.free + full - 1 - (b ? take_end[b - 1] : 0) - (block - held));
+  a.seq[i] = b, a.pos[i] = pos, a.slot[i] = (long long)page * a.page + (pos - block * a.page);
+}
 
 __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTables a) {
   extern __shared__ int st_smem[];
@@ -73,36 +96,35 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
       if (bad) n = 0;
       else {
         start = out ? 0 : (int)len;
-        gone = out ? st_pages(len, a.page) : 0;
-        need = st_pages(start + n, a.page) - st_pages(start, a.page);
+        gone = out ? st_pages((int)len, a.page) : 0;
+        need = st_pages(start + (int)n, a.page) - st_pages(start, a.page);
       }
     }
     long long r = n;
     int p = gone, t = need;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long r2 = __shfl_up_sync(0xffffffffu, r, o);
-      const int p2 = __shfl_up_sync(0xffffffffu, p, o), t2 = __shfl_up_sync(0xffffffffu, t, o);
-      if (lane >= o) r += r2, p += p2, t += t2;
-    }
+    st_scan(r, p, t, lane);
     __syncthreads();                                       // bad_bits is set, the sums of the requests before are read
     if (bad) atomicOr(&bad_bits, bad);
     if (lane == 31) warp_rows[warp] = r, warp_push[warp] = p, warp_take[warp] = t;
     __syncthreads();
-    long long all_r = rows;
-    int all_p = push, all_t = take;
-#pragma unroll
-    for (int w = 0; w < 32; ++w) {
-      if (w == warp) r += all_r, p += all_p, t += all_t;
-      all_r += warp_rows[w], all_p += warp_push[w], all_t += warp_take[w];
-    }
+    // every warp sums up the warps' totals for itself
+    long long wr = warp_rows[lane];
+    int wp = warp_push[lane], wt = warp_take[lane];
+    st_scan(wr, wp, wt, lane);
+    const int before = max(warp - 1, 0);
+    const long long br = __shfl_sync(0xffffffffu, wr, before);
+    const int bp = __shfl_sync(0xffffffffu, wp, before), bt = __shfl_sync(0xffffffffu, wt, before);
+    r += rows, p += push, t += take;
+    if (warp > 0) r += br, p += bp, t += bt;
+    rows += __shfl_sync(0xffffffffu, wr, 31);
+    push += __shfl_sync(0xffffffffu, wp, 31);
+    take += __shfl_sync(0xffffffffu, wt, 31);
     if (b < a.B) {
       row_end[b] = (int)min(r, 0x7fffffffll);
       push_end[b] = p;
       take_end[b] = t;
       base[b] = start;
     }
-    rows = all_r, push = all_p, take = all_t;
   }
   __syncthreads();
   int bad = bad_bits;
@@ -115,9 +137,14 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
       const int b = st_owner(push_end, a.B, i);
       a.free[top + i] = a.bt[b * a.bt_stride + push_end[b] - 1 - i];
     }
-  __threadfence();
-  cluster_arrive();
-  cluster_wait();
+  // what is pushed is there for every CTA, and all inputs are read, before anything else is written
+  if (ctas > 1) {
+    if (push > 0) __threadfence();
+    cluster_arrive();
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
   const int full = top + push;
   if (rank == 0) {
     for (int b = tid; b < a.B; b += ST_THREADS) {
@@ -138,15 +165,23 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
       const int nth = i - (b ? take_end[b - 1] : 0);
       a.bt[b * a.bt_stride + st_pages(base[b], a.page) + nth] = stack[full - 1 - i];
     }
-  for (int i = at; i < a.rows; i += step) {
-    if (bad || i >= rows) {
-      a.seq[i] = 0, a.pos[i] = 0, a.slot[i] = -1;
-      continue;
+  // PER rows in a run for each thread: one bisection, and mostly one page
+  constexpr int PER = 4;
+  const int runs = (a.rows + PER - 1) / PER, live = bad ? 0 : (int)rows;
+  if (a.rows <= 2 * step) {
+    for (int i = at; i < a.rows; i += step) st_row(a, i, i < live ? st_owner(row_end, a.B, i) : -1, row_end, take_end, base, full);
+    return;
+  }
+  for (int run = at; run < runs; run += step) {
+    int i = run * PER, b = i < live ? st_owner(row_end, a.B, i) : -1;
+#pragma unroll
+    for (int k = 0; k < PER; ++k, ++i) {
+      if (i >= a.rows) break;
+      if (i >= live) b = -1;
+      else
+        while (row_end[b] <= i) ++b;
+      st_row(a, i, b, row_end, take_end, base, full);
     }
-    const int b = st_owner(row_end, a.B, i), pos = base[b] + i - (b ? row_end[b - 1] : 0);
-    const int held = st_pages(base[b], a.page), block = pos / a.page;
-    const int page = block < held ? a.bt[b * a.bt_stride + block] : stack[full - 1 - (b ? take_end[b - 1] : 0) - (block - held)];
-    a.seq[i] = b, a.pos[i] = pos, a.slot[i] = (long long)page * a.page + pos % a.page;
   }
 }
 

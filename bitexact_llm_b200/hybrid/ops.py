@@ -220,12 +220,17 @@ def gqa_cache4(spec, n_blocks, page, dev):
     """An empty cache of keys and values in 4 bits (its form: include/bitexact_float.h) for pages of `page` tokens, a multiple of 64."""
     if page < 1 or page % CACHE4_TOKENS:
         raise ValueError(f"the 4-bit cache has pages of multiples of {CACHE4_TOKENS} tokens, not {page}")
-    return torch.zeros(n_blocks, spec.kv_heads, page // CACHE4_TOKENS, nv.float_lib().bxf_cache4_block(spec.dim, spec.vdim),
+    return torch.zeros(n_blocks, spec.kv_heads, page // CACHE4_TOKENS, _block4(spec.dim, spec.vdim),
                        dtype=torch.uint8, device=dev)
 
 
+def _block4(dim, vdim):
+    """bxf_cache4_block."""
+    return 36 * ((dim + 63) // 64 + (vdim + 63) // 64) * 64 + 2 * CACHE4_TOKENS
+
+
 def _check4(cache, dim, vdim):
-    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.shape[3] != nv.float_lib().bxf_cache4_block(dim, vdim):
+    if cache.dtype != torch.uint8 or cache.dim() != 4 or not cache.is_contiguous() or cache.shape[3] != _block4(dim, vdim):
         raise ValueError(f"not a 4-bit cache for keys of {dim} and values of {vdim} entries")
 
 
@@ -267,7 +272,7 @@ def gqa_attention4(q, spec, cache, bt, seq, pos, sink, tiles=None, variant=0):
         raise ValueError("gqa_attention4: queries T [kv_heads, M, heads per group, >= dim], contiguous")
     if bt.dtype not in (torch.int32, torch.int64) or bt.dim() != 2 or bt.shape[1] > 1 and bt.stride(1) != 1:
         raise ValueError("gqa_attention4: bt int32 or int64 [sequences, blocks], rows contiguous")
-    if any(t.dtype != torch.int64 or t.shape != (M,) or not t.is_contiguous() for t in (seq, pos)):
+    if seq.dtype != torch.int64 or pos.dtype != torch.int64 or seq.shape != (M,) or pos.shape != (M,) or not (seq.is_contiguous() and pos.is_contiguous()):
         raise ValueError("gqa_attention4: seq and pos int64 [M]")
     if tiles is not None and (tiles.dtype != torch.int32 or tiles.dim() != 2 or tiles.shape[1] != 3 or not tiles.is_contiguous()):
         raise ValueError("gqa_attention4: tiles int32 [T, 3]")

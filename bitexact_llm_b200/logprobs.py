@@ -39,11 +39,12 @@ def log_probs(logits, tokens=None, top=0, fr=24):
     if not 0 <= top <= MAX_TOP or not 0 <= fr <= 40:
         raise ValueError(f"log_probs: top is 0 .. {MAX_TOP}, fr 0 .. 40")
     nv.here(logits, tokens)
-    dev = logits.device
-    tokens = None if tokens is None else tokens.contiguous()
-    logp, entropy, top_logp = (torch.empty(*s, dtype=torch.float32, device=dev) for s in ((n,), (n,), (n, top)))
-    rank, top_ids = torch.empty(n, dtype=torch.int64, device=dev), torch.empty(n, top, dtype=torch.int64, device=dev)
+    dev, given = logits.device, tokens is not None
+    tokens = tokens.contiguous() if given else None
+    # the outputs are parts of two buffers: an allocation each costs more than a small call
+    logp, entropy, top_logp = torch.empty(2 * n + n * top, dtype=torch.float32, device=dev).split_with_sizes((n, n, n * top))
+    rank, top_ids = torch.empty(n + n * top, dtype=torch.int64, device=dev).split_with_sizes((n, n * top))
     rc = nv.lib().bx_log_probs(KINDS[logits.dtype], logits.data_ptr(), logits.stride(0) if n > 1 else V, nv.ptr(tokens), top, logp.data_ptr(),
                                entropy.data_ptr(), rank.data_ptr(), top_ids.data_ptr(), top_logp.data_ptr(), n, V, fr, nv.stream())
     nv.check(rc, "bx_log_probs")
-    return LogProbs(None if tokens is None else logp, entropy, None if tokens is None else rank, top_ids, top_logp)
+    return LogProbs(logp if given else None, entropy, rank if given else None, top_ids.view(n, top), top_logp.view(n, top))

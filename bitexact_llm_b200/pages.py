@@ -24,6 +24,10 @@ class StepTables(NamedTuple):
     status: torch.Tensor        # int32 [1]: 0, or why nothing was done
 
 
+def _whole(t, shape, dtype=torch.int64):
+    return t.dtype == dtype and t.shape == shape and t.is_contiguous()
+
+
 def step_tables(lens, counts, bt, free, top, page, rows, drop=None, lens_out=None, top_out=None, status=None):
     """lens, counts int64 [B]: tokens in the cache and new ones; bt int32 [B, blocks] (extended in place); free int32 [pool], top
     int32 [1]: the stack of free pages, of which the first `top` are there (its end is written in place); rows: token rows that the
@@ -32,28 +36,29 @@ def step_tables(lens, counts, bt, free, top, page, rows, drop=None, lens_out=Non
     lens_out, top_out: where the state behind the step goes (may be lens and top; default: new tensors, so that the same call again
     gives the same rows). status: an int32 [1] to which this call's bits are added (default: a new one). Bits: TOO_LONG, NO_PAGES,
     TOO_MANY_ROWS, INVALID; with any of them no page changes hands and all rows are padding."""
-    B = lens.shape[0] if lens.dim() == 1 else -1
-    if any(t.dtype != torch.int64 or t.shape != (B,) or not t.is_contiguous() for t in (lens, counts, *(() if lens_out is None else (lens_out,)))):
+    shape, i32 = lens.shape, torch.int32
+    if lens.dim() != 1 or not (_whole(lens, shape) and _whole(counts, shape)) or lens_out is not None and not _whole(lens_out, shape):
         raise ValueError("step_tables: lens and counts int64 [B], contiguous")
-    if bt.dtype != torch.int32 or bt.dim() != 2 or bt.shape[0] != B or bt.shape[1] < 1 or bt.shape[1] > 1 and bt.stride(1) != 1 or B > 1 and bt.stride(0) < bt.shape[1]:
+    B, (stride, unit) = shape[0], bt.stride() if bt.dim() == 2 else (0, 0)
+    if bt.dtype != i32 or bt.dim() != 2 or bt.shape[0] != B or bt.shape[1] < 1 or bt.shape[1] > 1 and unit != 1 or B > 1 and stride < bt.shape[1]:
         raise ValueError("step_tables: bt int32 [B, blocks], rows contiguous")
-    if free.dtype != torch.int32 or free.dim() != 1 or not free.is_contiguous():
+    if free.dtype != i32 or free.dim() != 1 or not free.is_contiguous():
         raise ValueError("step_tables: free int32 [pool], contiguous")
-    if any(t.dtype != torch.int32 or t.numel() != 1 for t in (top, *(t for t in (top_out, status) if t is not None))):
+    if top.dtype != i32 or top.numel() != 1 or any(t is not None and (t.dtype != i32 or t.numel() != 1) for t in (top_out, status)):
         raise ValueError("step_tables: top and status int32 [1]")
-    if drop is not None and (drop.dtype != torch.bool or drop.shape != (B,) or not drop.is_contiguous()):
+    if drop is not None and not _whole(drop, shape, torch.bool):
         raise ValueError("step_tables: drop bool [B], contiguous")
     if page < 1 or rows < 0 or B > MAX_REQUESTS:
         raise ValueError(f"step_tables: pages of at least one token, at most {MAX_REQUESTS} requests")
     nv.here(lens, counts, bt, free, top, drop, lens_out, top_out, status)
-    dev = lens.device
-    seq, pos, slot = torch.empty(3, rows, dtype=torch.int64, device=dev).unbind(0)
-    last = torch.empty(B, dtype=torch.int64, device=dev)
-    lens_out = torch.empty_like(lens) if lens_out is None else lens_out
-    top_out = torch.empty_like(top) if top_out is None else top_out
     sticky = status is not None
-    status = status if sticky else torch.empty(1, dtype=torch.int32, device=dev)
-    rc = nv.lib().bx_step_tables(lens.data_ptr(), counts.data_ptr(), nv.ptr(drop), bt.data_ptr(), bt.stride(0) if B > 1 else bt.shape[1],
+    # the outputs are parts of two buffers: an allocation each costs more than the kernel
+    seq, pos, slot, last, out = torch.empty(3 * rows + 2 * B, dtype=torch.int64, device=lens.device).split_with_sizes((rows, rows, rows, B, B))
+    lens_out = out if lens_out is None else lens_out
+    if top_out is None or status is None:
+        a, b = torch.empty(2, dtype=i32, device=lens.device).split_with_sizes((1, 1))
+        top_out, status = a if top_out is None else top_out, b if status is None else status
+    rc = nv.lib().bx_step_tables(lens.data_ptr(), counts.data_ptr(), nv.ptr(drop), bt.data_ptr(), stride if B > 1 else bt.shape[1],
                                  bt.shape[1], page, free.data_ptr(), free.shape[0], top.data_ptr(), B, rows, seq.data_ptr(), pos.data_ptr(),
                                  slot.data_ptr(), last.data_ptr(), lens_out.data_ptr(), top_out.data_ptr(), status.data_ptr(), int(sticky),
                                  nv.stream())
