@@ -183,7 +183,7 @@ _FLOAT_SIGNATURES = {
     "bxf_cache4_block": (Z, [I, I]),
     "bxf_gqa_store4": (I, [I, P, L, L, P, L, L, P, I, I, I, I, P, I, I, P]),
     "bxf_gqa_read4": (I, [I, P, I, I, I, I, I, P, P, P, I, P]),
-    "bxf_gqa_attention4": (I, [I, P, L, I, I, I, I, I, P, I, I, P, I, L, I, P, P, P, I, I, P, R, P, L, I, P]),
+    "bxf_gqa_attention4": (I, [I, P, L, I, I, I, I, I, P, I, I, P, I, L, I, P, P, P, I, I, P, R, P, L, P, Z, I, P]),
     "bxf_streams": (I, [I, ctypes.POINTER(StreamsStep), I, P]),
     "bxf_causal_conv": (I, [I, ctypes.POINTER(Conv), P, L, I, P]),
     "bxf_recurrence": (I, [I, ctypes.POINTER(RecurrenceRows), I, P]),

@@ -183,7 +183,7 @@ __host__ __device__ constexpr int a4_ring_bytes() {
 }
 
 template <int K, int V, int NT>
-__global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_kernel(const PagedAttn a, const Cache4 c) {
+__global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_kernel(const PagedAttn a, const Cache4 c, int max_rows) {
   constexpr int BYTES = a4_block_bytes<K, V>(), KS = K / 16, KW = K / 32, ROWS = 8 * NT;
   extern __shared__ __align__(128) uint8_t a4_raw[];
   uint8_t* ring_all = a4_raw;
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
     seq = a.seq[tok0];
   }
   const int row0 = blockIdx.z * ROWS, rows = min(ROWS, ntok * a.H - row0);
-  if (rows <= 0) return;                                   // all CTAs of the cluster alike
+  if (rows <= 0 || a.tiles && ntok * a.H > max_rows) return;             // all CTAs of the cluster alike; taller tiles are another kernel's
   const i64 limit = (i64)a.nblk * a.bs - 1;
   const int t_first = row0 / a.H, t_last = (row0 + rows - 1) / a.H;
   const i64 p_first = min(a.pos[tok0 + t_first], limit), p_last = min(a.pos[tok0 + t_last], limit);

@@ -14,9 +14,15 @@
 // so that two CTAs share an SM and the scores -> softmax -> values chain of one tile runs beside the other's. The running maximum starts at the sink (denominator 1); the accumulator is rescaled only when the maximum
 // grows by more than 2^8 since the last time. Few tiles (decoding): the keys of a tile are split over blockIdx.y, and a
 // second kernel joins the parts.
+//
+// A 4-bit cache (FOUR; fl_cache4.cuh) has two more warps, which make the bf16 operands of a block in shared memory from its codes: a raw
+// block arrives by one bulk copy while the warps wait for a free stage, keys become K-major rows as a TMA copy would leave them,
+// values, whose codes lie along the tokens, a K-major V^T. Entries are exact in bf16, so everything behind the operands is the same
+// kernel. It is for tiles of many query rows, which share that work; short tiles have the kernel of fl_attention4.cuh, and each of
+// the two leaves the other's tiles alone.
 #pragma once
 
-#include "fl_attention.cuh"
+#include "fl_attention4.cuh"
 #include "fl_gemm.cuh"
 
 namespace bxf {
@@ -32,11 +38,12 @@ struct LatentTc {
   int row_blocks, vsplit;                                // blockIdx.z = (group * vsplit + value slice) * row_blocks + row block
   int splits;
   float* part;                                           // splits > 1: [splits][M G H][R] accumulators, then [splits][M G H][2]
+  int min_rows;                                          // FOUR: tiles of fewer query rows are another kernel's
 };
 
 struct LatentShared {
   uint64_t q_full, o_done;
-  uint64_t full[LT_MAX_STAGES], empty[LT_MAX_STAGES];
+  uint64_t full[LT_MAX_STAGES], empty[LT_MAX_STAGES], raw_full;
   uint64_t s_full[2], p_full[2], pv_done[2];
   float row_max[2][4][128], row_den[4][128];
   uint32_t tmem_base, abort_flag;
@@ -53,7 +60,85 @@ template <int PARTS>
 __device__ __forceinline__ void quarter_barrier(int quarter) {
   asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * PARTS) : "memory");
 }
-__host__ __device__ constexpr int lt_threads(int parts) { return 64 + 128 * parts; }
+constexpr int LT_LOADERS = 2;                            // warps that make operands from codes
+__host__ __device__ constexpr int lt_threads(int parts, bool four = false) { return 64 + 128 * parts + (four ? 32 * LT_LOADERS : 0); }
+
+__device__ __forceinline__ void loaders_barrier() { asm volatile("bar.sync 9, %0;" ::"n"(32 * LT_LOADERS) : "memory"); }
+
+// fp16 products of a code and its scale (normal or zero) -> bf16, times the powers of two in `power`, 2^(112 + e): an fp16 number shifted
+// down by three bits is the bf16 of its 2^-112-fold. `high`: powers beyond that range, for the lanes that need them.
+__device__ __forceinline__ uint32_t bf16_of(uint32_t h, uint32_t power) {
+  const uint32_t t = (h >> 3 & 0x0fff0fffu) | (h & 0x80008000u);
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(power));
+  return r;
+}
+// 2^(112 + e) as bf16 in both halves from two exponent bytes e + 127 (in the low bytes of w's halves); up to e = 15.
+__device__ __forceinline__ uint32_t bf16_powers(uint32_t w) { return (w + 0x00700070u) << 7; }
+
+// One block's keys, by all loader threads: thread (row, column box) writes 64 entries of a row, 16 bytes at a time where a
+// 128-byte-swizzled copy would put them.
+__device__ __forceinline__ void operand_keys(const uint8_t* raw, uint8_t* st, const Cache4& c, int tid) {
+  for (int u = tid; u < LT_KEYS * (c.K / 64); u += 32 * LT_LOADERS) {
+    const int r = u % LT_KEYS, box = u / LT_KEYS, e = raw[c.key_exp(r)];
+    const uint32_t finite = bf16_powers(min(e, 142) * 0x00010001u), more = (uint32_t)(e > 142 ? e - 142 + 127 : 127) * 0x00800080u;
+    const uint4* codes = reinterpret_cast<const uint4*>(raw + r * (c.K / 2) + box * 32);
+    uint8_t* row = st + box * (LT_KEYS * 128) + r * 128;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint4 v = codes[half];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {                      // 8 codes: a chunk of 16 bytes
+        const uint32_t byte = raw[c.key_scale(r, box * 4 + half * 2 + k / 2)] & 127, scale = e4m3_pair(byte * 0x0101u);
+        const uint32_t power = byte == C4_NAN ? 0x7fff7fffu : finite;
+        uint32_t h[4];
+        e2m1_pairs(w[k], h);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          h[x] = bf16_of(hmul2(h[x], scale), power);
+          if (e > 142) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(h[x]) : "r"(more));
+        }
+        *reinterpret_cast<uint4*>(row + (((half * 4 + k) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+  }
+}
+// Its values as V^T: thread (byte column, 16 tokens) writes two runs of 16 tokens, of entries 16 j + i and 16 j + i + 8.
+__device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, const Cache4& c, int tid) {
+  for (int u = tid; u < c.V / 2 * 4; u += 32 * LT_LOADERS) {
+    const int col = u % (c.V / 2), t0 = u / (c.V / 2) * 16, j = col / 8, i = col % 8;
+    const uint4 vc = *reinterpret_cast<const uint4*>(raw + 36 * c.K + col * C4_TOKENS + t0);
+    const uint4 vs = *reinterpret_cast<const uint4*>(raw + 36 * c.K + 32 * c.V + j * C4_TOKENS + t0);
+    const uint4 ve = *reinterpret_cast<const uint4*>(raw + 36 * (c.K + c.V) + C4_TOKENS + t0);
+    const uint32_t cw[4] = {vc.x, vc.y, vc.z, vc.w}, sw[4] = {vs.x, vs.y, vs.z, vs.w}, ew[4] = {ve.x, ve.y, ve.z, ve.w};
+    uint32_t lo[8], hi[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {                        // 4 tokens
+      uint32_t h[4];
+      e2m1_pairs(cw[q], h);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t scale = e4m3_pair(sw[q] >> (16 * x)), e = __byte_perm(ew[q], 0, x ? 0x4342 : 0x4140);
+        const uint32_t power = bf16_powers(__vminu2(e, 0x008e008eu));
+        lo[2 * q + x] = bf16_of(hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), scale), power);
+        hi[2 * q + x] = bf16_of(hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), scale), power);
+        if (__vmaxu2(e, 0x008e008eu) != 0x008e008eu) {
+          const uint32_t more = (__vmaxu2(e, 0x008e008eu) - 0x000f000fu) << 7;
+          asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(lo[2 * q + x]) : "r"(more));
+          asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(hi[2 * q + x]) : "r"(more));
+        }
+      }
+    }
+    uint8_t* row = st + (16 * j + i) * 128;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int at = (t0 / 8 + k ^ i) << 4;              // 16 j + i and + 8 are alike modulo 8
+      *reinterpret_cast<uint4*>(row + at) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+      *reinterpret_cast<uint4*>(row + 8 * 128 + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+    }
+  }
+}
 
 // D (+)= A[tmem] * B[smem]; A: bf16 pairs, one row per lane.
 __device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -76,10 +161,10 @@ __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t addr) {
   return d | static_cast<uint64_t>((LT_KEYS * 128) >> 4) << 16;
 }
 
-template <int PARTS>
-__global__ void __launch_bounds__(lt_threads(PARTS), PARTS == 2 ? 2 : 1)
+template <int PARTS, bool FOUR = false>
+__global__ void __launch_bounds__(lt_threads(PARTS, FOUR), PARTS == 2 ? 2 : 1)
 fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mc,
-                             const PagedAttn a, const LatentTc c) {
+                             const PagedAttn a, const LatentTc c, const Cache4 c4) {
   constexpr int TCOLS = PARTS == 2 ? 256 : 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* qs = align_smem(smem_raw);
@@ -87,6 +172,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
   uint8_t* ring = qs + c.kcols * q_box;
   const int stage_bytes = c.cols * LT_KEYS * 128;
   LatentShared* sh = reinterpret_cast<LatentShared*>(ring + c.stages * stage_bytes);
+  uint8_t* raw = reinterpret_cast<uint8_t*>(sh) + (sizeof(LatentShared) + 15) / 16 * 16;           // FOUR: a block as it is in the cache
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   wait_previous();
@@ -113,15 +199,17 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
   const int b0 = b_lo + (b_hi - b_lo) * (int)blockIdx.y / c.splits, b1 = b_lo + (b_hi - b_lo) * ((int)blockIdx.y + 1) / c.splits;
   const int nb = b1 - b0;
   if (rows <= 0) return;
+  if (FOUR && ntok * a.H < c.min_rows) return;
   const int quarters = (rows + 31) / 32;                 // TMEM lane quarters in use
 
   if (threadIdx.x == 0) {
     mbar_init(&sh->q_full, 1);
     mbar_init(&sh->o_done, 1);
     for (int i = 0; i < c.stages; ++i) {
-      mbar_init(&sh->full[i], 1);
+      mbar_init(&sh->full[i], FOUR ? LT_LOADERS : 1);
       mbar_init(&sh->empty[i], 1);
     }
+    mbar_init(&sh->raw_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], PARTS * quarters);
@@ -163,7 +251,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       const int box = min(a.bs, LT_KEYS), boxes = LT_KEYS / box;
       int i = 0, held = 0;
       bool ok = true;
-      for (; i < nb; ++i) {
+      for (; !FOUR && i < nb; ++i) {
         const int s = i % c.stages, round = i / c.stages;
         if (round > 0) ok = mbar_wait(&sh->empty[s], (round - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -194,7 +282,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       // ---- MMA: scores of block i + 1 are issued before the values of block i. A query box of fewer than 128 rows is
       //      read on into what follows it in shared memory: those accumulator lanes belong to no query ----
       constexpr uint32_t ID_S = umma_idesc_bf16(LT_KEYS);
-      const uint32_t id_v = umma_idesc_bf16((vn + 15) / 16 * 16, true);
+      const uint32_t id_v = umma_idesc_bf16((vn + 15) / 16 * 16, !FOUR);
       auto scores = [&](int i) {
         const int s = i % c.stages, buf = i & 1;
         if (!mbar_wait(&sh->full[s], (i / c.stages) & 1)) return false;
@@ -218,13 +306,47 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         const uint32_t va = smem_u32(ring + s * stage_bytes) + (c.vbox + v0 / 64) * LT_KEYS * 128;
 #pragma unroll
         for (int ks = 0; ks < LT_KEYS / 16; ++ks)
-          umma_bf16_ts(tmem + LT_O, tmem + buf * LT_KEYS + ks * 8, umma_desc_mn(va + ks * 2048), id_v, (i | ks) != 0);
+          umma_bf16_ts(tmem + LT_O, tmem + buf * LT_KEYS + ks * 8, FOUR ? umma_desc_sw128(va + ks * 32) : umma_desc_mn(va + ks * 2048), id_v, (i | ks) != 0);
         umma_commit(&sh->pv_done[buf]);
         umma_commit(&sh->empty[s]);
         if (c.stages == 1 && i + 1 < nb) ok = scores(i + 1);             // one stage: nothing to run ahead into
       }
       if (ok) umma_commit(&sh->o_done);
       else fail();
+    }
+  } else if (FOUR && warp >= 2 + 4 * PARTS) {
+    // ---- operands from codes: the raw block of the next step is fetched as soon as this one's is used ----
+    const int tid = threadIdx.x - 32 * (2 + 4 * PARTS), bytes = c4.bytes(), in_page = a.bs / LT_KEYS;
+    int held = 0;
+    auto fetch = [&](int i) {                            // the first warp reads the block table for 32 blocks at a time
+      if (warp != 2 + 4 * PARTS) return;
+      if ((i & 31) == 0) held = (int)a.page_of(seq, min((b0 + i + lane) / in_page, a.nblk - 1));
+      const i64 page = __shfl_sync(0xffffffffu, held, i & 31);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&sh->raw_full, bytes);
+        bulk_load(raw, c4.p + ((page * a.G + group) * in_page + (b0 + i) % in_page) * bytes, &sh->raw_full, bytes);
+      }
+    };
+    if (nb > 0) fetch(0);
+    // a wait that gives up is remembered and the loop goes on, without waits, copies or work: the barrier counts both warps
+    bool ok = true;
+    for (int i = 0; i < nb; ++i) {
+      const int s = i % c.stages, round = i / c.stages;
+      if (ok) {
+        ok = mbar_wait(&sh->raw_full, i & 1) && (round == 0 || mbar_wait(&sh->empty[s], (round - 1) & 1));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok && lane == 0) fail();
+      }
+      if (ok) {
+        uint8_t* st = ring + s * stage_bytes;
+        operand_keys(raw, st, c4, tid);
+        operand_values(raw, st + c.kcols * LT_KEYS * 128, c4, tid);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->full[s]);
+      }
+      loaders_barrier();                                 // the raw block is read
+      if (ok && i + 1 < nb) fetch(i + 1);
     }
   } else if ((warp & 3) < quarters) {
     // ---- softmax. A wait that gives up is remembered and the loop goes on (the quarter's barriers count every warp) ----

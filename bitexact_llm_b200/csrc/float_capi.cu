@@ -278,7 +278,7 @@ int launch_paged_tc(const PagedAttn& a, void* scratch, size_t scratch_bytes, cud
     return BX_ELAUNCH;
   const dim3 grid(tiles, c.splits, c.row_blocks * c.vsplit * a.G);
   const int rc = launch_chained(fl_paged_attention_tc_kernel<PARTS>, grid, lt_threads(PARTS), fixed + c.stages * c.cols * LT_KEYS * 128, st,
-                                0, mq, mc, a, c);
+                                0, mq, mc, a, c, Cache4{});
   if (rc != BX_OK || c.splits == 1) return rc;
   return launch_chained(fl_attention_join_kernel, dim3((unsigned)(a.M * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits);
 }
@@ -327,7 +327,7 @@ int attention4_cluster(i64 tiles, i64 blocks, int per_sm) {
 }
 
 template <int K, int V, int NT>
-int launch_attention4(const PagedAttn& a, const Cache4& c, cudaStream_t st) {
+int launch_attention4(const PagedAttn& a, const Cache4& c, int most, cudaStream_t st) {
   constexpr int smem = a4_ring_bytes<K, V, NT>() + sizeof(A4Shared), per_sm = NT == 1 ? 3 : 2;
   static PerDevice configured;
   if (once_per_device(configured, [] {
@@ -335,21 +335,68 @@ int launch_attention4(const PagedAttn& a, const Cache4& c, cudaStream_t st) {
         return e != cudaSuccess ? e : cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       }) != BX_OK)
     return BX_ELAUNCH;
-  const int n = a.tiles ? a.ntiles : a.M, rows = a.tiles ? (a.H > 128 ? a.H : 128) : a.H, z = ceil_div(rows, 8 * NT);
+  const int n = a.tiles ? a.ntiles : a.M, tallest = a.tiles ? (a.H > 128 ? a.H : 128) : a.H, rows = tallest < most ? tallest : most;
+  const int z = ceil_div(rows, 8 * NT);
   const int cluster = attention4_cluster((i64)n * a.G * z, (i64)a.nblk * a.bs / C4_TOKENS, per_sm);
-  return launch_chained(fl_attention4_kernel<K, V, NT>, dim3((unsigned)n * cluster, a.G, z), 32 * A4_WARPS, smem, st, cluster, a, c);
+  return launch_chained(fl_attention4_kernel<K, V, NT>, dim3((unsigned)n * cluster, a.G, z), 32 * A4_WARPS, smem, st, cluster, a, c, most);
 }
 
 template <int NT>
-int launch_attention4(const PagedAttn& a, const Cache4& c, cudaStream_t st) {
-  if (c.K == 64) return c.V == 64 ? launch_attention4<64, 64, NT>(a, c, st) : launch_attention4<64, 128, NT>(a, c, st);
-  return c.V == 64 ? launch_attention4<128, 64, NT>(a, c, st) : launch_attention4<128, 128, NT>(a, c, st);
+int launch_attention4(const PagedAttn& a, const Cache4& c, int most, cudaStream_t st) {
+  if (c.K == 64) return c.V == 64 ? launch_attention4<64, 64, NT>(a, c, most, st) : launch_attention4<64, 128, NT>(a, c, most, st);
+  return c.V == 64 ? launch_attention4<128, 64, NT>(a, c, most, st) : launch_attention4<128, 128, NT>(a, c, most, st);
 }
 
-int run_attention4(int dtype, const PagedAttn& a, const Cache4& c, int variant, cudaStream_t st) {
+// Tall tiles over a 4-bit cache on tcgen05, two CTAs per SM; the keys are split only as in launch_paged_tc.
+int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, void* scratch, size_t scratch_bytes, cudaStream_t st) {
+  static PerDevice configured;
+  if (once_per_device(configured, [] {
+        return cudaFuncSetAttribute(fl_paged_attention_tc_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, LT_PAIR_SMEM);
+      }) != BX_OK)
+    return BX_ELAUNCH;
+  LatentTc c = {};
+  c.kcols = c.vbox = c4.K / 64;
+  c.cols = c.kcols + c4.V / 64;
+  c.min_rows = min_rows;
+  const int tokens = bxf_latent_attention_tile(a.H), rows = tokens * a.H;
+  c.qrows = rows >= 128 ? 128 : ceil_div(rows, 8) * 8;
+  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared) + 16 + c4.bytes();
+  c.stages = (LT_PAIR_SMEM - fixed) / (c.cols * LT_KEYS * 128);
+  if (c.stages > LT_MAX_STAGES) c.stages = LT_MAX_STAGES;
+  c.row_blocks = ceil_div(rows, 128);
+  c.vsplit = 1;
+  c.splits = 1;
+  const i64 span = a.window > 0 && a.window + tokens < (i64)a.nblk * a.bs ? a.window + tokens : (i64)a.nblk * a.bs;
+  const i64 blocks = span / LT_KEYS + 1, ctas = (i64)a.ntiles * c.row_blocks * a.G;
+  if ((i64)c.row_blocks * a.G > 65535) return BX_ELIMIT;
+  const int sms = device_sms();
+  if (sms <= 0) return BX_ELAUNCH;
+  while (c.splits < LT_MAX_SPLIT && ctas * c.splits * 2 <= sms && blocks >= c.splits * 4 && scratch &&
+         scratch_bytes >= attention_scratch((i64)a.M * a.H * a.G, a.R, c.splits * 2))
+    c.splits *= 2;
+  c.part = static_cast<float*>(scratch);
+  CUtensorMap mq;
+  if (!make_map_bf16(&mq, a.q, a.W, (i64)a.M * a.H, a.G, a.ldq, (i64)a.M * a.H * a.ldq, c.qrows, 1)) return BX_ELAUNCH;
+  const int rc = launch_chained(fl_paged_attention_tc_kernel<2, true>, dim3(a.ntiles, c.splits, c.row_blocks * a.G), lt_threads(2, true),
+                                fixed + c.stages * c.cols * LT_KEYS * 128, st, 0, mq, mq, a, c, c4);
+  if (rc != BX_OK || c.splits == 1) return rc;
+  // it writes every row; those of short tiles get what is theirs from the kernel behind it
+  return launch_chained(fl_attention_join_kernel, dim3((unsigned)(a.M * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits);
+}
+
+int run_attention4(int dtype, const PagedAttn& a, const Cache4& c, void* scratch, size_t scratch_bytes, int variant, cudaStream_t st) {
   const bool fits = attention4_fits(dtype, c) && (!a.tiles || a.ntiles > 0) && a.G <= 65535;
-  if (variant == 2 && !fits) return BX_ELIMIT;
-  if (variant != 1 && fits) return a.tiles || a.H > 8 ? launch_attention4<2>(a, c, st) : launch_attention4<1>(a, c, st);
+  const int groups = a.H <= 8 ? 1 : 2, few = 8 * groups;                             // query rows that one warp takes
+  const bool tall = a.tiles && aligned16(a.q) && a.ldq % 8 == 0;                       // (a TMA copy of the queries)
+  if (variant >= 2 && !fits) return BX_ELIMIT;
+  if (variant != 1 && fits) {
+    if (tall && variant != 2) {
+      const int rc = launch_attention4_tc(a, c, few + 1, scratch, scratch_bytes, st);
+      if (rc != BX_OK || a.H > few) return rc;
+    }
+    const int most = tall && variant != 2 ? few : 0x7fffffff;
+    return groups == 1 && (!a.tiles || most == few) ? launch_attention4<1>(a, c, most, st) : launch_attention4<2>(a, c, most, st);
+  }
   const dim3 grid(a.M, a.H * a.G);
   const int smem = (c.K + 2 * c.V) * 4;
   if (dtype == BXF_F32) return launch_chained(fl_attention4_plain_kernel<float>, grid, A4_THREADS, smem, st, 0, a, c);
@@ -730,10 +777,10 @@ int bxf_gqa_read4(int dtype, const void* cache, int kv_heads, int dim, int vdim,
 
 int bxf_gqa_attention4(int dtype, const void* q, int64_t ldq, int M, int heads, int kv_heads, int dim, int vdim, const void* cache, int page,
                        int nb, const void* bt, int bt_is64, int64_t bt_stride, int nblk, const int64_t* seq, const int64_t* pos,
-                       const int* tiles, int ntiles, int window, const float* sink, float scale, void* out, int64_t ldo, int variant,
-                       void* stream) {
+                       const int* tiles, int ntiles, int window, const float* sink, float scale, void* out, int64_t ldo, void* scratch,
+                       size_t scratch_bytes, int variant, void* stream) {
   if (!dtype_ok(dtype) || M < 0 || heads < 1 || !cache4_ok(cache, kv_heads, dim, vdim, page, nb) || heads % kv_heads || ldq < dim ||
-      ldo < (int64_t)heads * vdim || nblk < 1 || window < 0 || ntiles < 0 || variant < 0 || variant > 2)
+      ldo < (int64_t)heads * vdim || nblk < 1 || window < 0 || ntiles < 0 || variant < 0 || variant > 3)
     return BX_EARG;
   if (dim > C4_MAX || vdim > C4_MAX || heads > 65535 || (i64)nblk * page > 0x3fffffff) return BX_ELIMIT;
   if (g_status_seen.load() != 0) return BX_EDEVICE;
@@ -742,7 +789,7 @@ int bxf_gqa_attention4(int dtype, const void* q, int64_t ldq, int M, int heads, 
   const Cache4 c = cache4_of(cache, kv_heads, dim, vdim, page, nb);
   const PagedAttn a{q, ldq, M, heads / kv_heads, kv_heads, dim, vdim, 0, cache, c.bytes(), page, nb, bt, bt_is64, bt_stride, nblk,
                     reinterpret_cast<const i64*>(seq), reinterpret_cast<const i64*>(pos), tiles, ntiles, window, sink, scale, out, ldo, vdim};
-  return run_attention4(dtype, a, c, variant, stream_of(stream));
+  return run_attention4(dtype, a, c, scratch, scratch_bytes, variant, stream_of(stream));
 }
 
 int bxf_streams(int dtype, const bxf_streams_step* p, int M, void* stream) {

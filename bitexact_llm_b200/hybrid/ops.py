@@ -280,11 +280,14 @@ def gqa_attention4(q, spec, cache, bt, seq, pos, sink, tiles=None, variant=0):
         raise ValueError("gqa_attention4: sink float32 [heads]")
     _check4(cache, dim, vdim)
     nv.here(q, cache, bt, seq, pos, sink, tiles)
+    lib = nv.float_lib()
     out = torch.empty(M, pad8(H * vdim), dtype=q.dtype, device=q.device)
-    rc = nv.float_lib().bxf_gqa_attention4(code(q), q.data_ptr(), ldq, M, H, G, dim, vdim, cache.data_ptr(), cache.shape[2] * CACHE4_TOKENS,
+    need = lib.bxf_gqa_attention_scratch(M, H, G, vdim) if tiles is not None else 0
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    rc = lib.bxf_gqa_attention4(code(q), q.data_ptr(), ldq, M, H, G, dim, vdim, cache.data_ptr(), cache.shape[2] * CACHE4_TOKENS,
                                            cache.shape[0], bt.data_ptr(), int(bt.dtype == torch.int64), bt.stride(0), bt.shape[1],
                                            seq.data_ptr(), pos.data_ptr(), nv.ptr(tiles), 0 if tiles is None else tiles.shape[0], spec.window,
-                                           nv.ptr(sink), spec.scale, out.data_ptr(), out.shape[1], variant, nv.stream())
+                                           nv.ptr(sink), spec.scale, out.data_ptr(), out.shape[1], nv.ptr(scratch), need, variant, nv.stream())
     nv.check(rc, "bxf_gqa_attention4")
     return out
 

@@ -6,7 +6,9 @@ e^s with |s| <= S give e^s (1 + (S + 2) 2^-23) on top, sums of n weights (n / 64
 output is off by less than 300 * 2^-24 * 60 * 2 ... of the largest |value|, 2.2e-3 at worst and in practice 1e-6; the tests hold the
 errors to `F32` = 3e-5 of the largest magnitude of a row's values, which random signs keep by far. bf16: weights are rounded to 11 bits (2^-12
 relative each, so the weighted mean moves by at most 2^-12 of the largest |value|, twice where the sum of the weights is not the rounded one's),
-the exponentials are off by 2^-21, the output by 2^-9: BF16 = 2^-11 of the largest |value| + 2^-8 of the output."""
+the exponentials are off by 2^-21, the output by 2^-8: 2^-11 of the largest |value| + 2^-8 of the output. The kernel of tall tiles holds weights in bf16,
+each off by at most half a step, 2^-8 of itself, while their sum is of the unrounded ones: the weighted mean moves by at most 2^-8 of the largest
+|value|, `TALL`, in place of 2^-11."""
 
 import math
 from types import SimpleNamespace
@@ -17,6 +19,7 @@ import torch
 pytestmark = pytest.mark.gpu
 DTYPES = ("bfloat16", "float32")
 F32 = 3e-5
+TALL = 2.0 ** -8
 GRID = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
 SCALES = torch.tensor([(c & 7) * 2.0 ** -9 if c < 8 else (8 + (c & 7)) * 2.0 ** ((c >> 3) - 10) for c in range(127)], dtype=torch.float64)
 
@@ -188,10 +191,10 @@ def attention(q, sp, seq, pos, held, sink):
     return out.flatten(1), big
 
 
-def close(got, want, big, dtype):
+def close(got, want, big, dtype, weights=2.0 ** -11):
     got = got.double().cpu()
     assert torch.isfinite(got).all()
-    tol = F32 * big if dtype == "float32" else 2.0 ** -11 * big + 2.0 ** -8 * want.abs()
+    tol = F32 * big if dtype == "float32" else weights * big + 2.0 ** -8 * want.abs()
     err = (got - want).abs()
     assert (err <= tol).all(), (float(err.max()), float((err / tol).max()))
 
@@ -203,7 +206,7 @@ def run(sp, page, lens, new, dtype, seed, sink=False, tiles=False, variant=0, bt
     t = tiles_of(new, sp.heads // sp.kv_heads) if tiles else None
     out = ops.gqa_attention4(q, sp, cache, bt.long() if bt64 else bt, seq, pos, s, t, variant)
     want, big = attention(q, sp, seq, pos, held, s)
-    close(out[:, : sp.heads * sp.vdim], want, big, dtype)
+    close(out[:, : sp.heads * sp.vdim], want, big, dtype, TALL if tiles and variant == 0 else 2.0 ** -11)
 
 
 VARIANTS = (0, 1)
@@ -232,12 +235,19 @@ def test_split_over_keys(batch_size, n, dtype):
     run(spec(8, 2, 128, 128), 64, [n] * batch_size, [1] * batch_size, dtype, n, sink=True)
 
 
-@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dtype,variant", [("bfloat16", 0), ("bfloat16", 1), ("bfloat16", 2), ("float32", 0)])
 @pytest.mark.parametrize("heads,kv_heads,dim,vdim,window", [(4, 1, 64, 64, 0), (8, 2, 128, 128, 0), (6, 2, 128, 64, 33), (5, 5, 20, 30, 0), (16, 1, 64, 128, 70),
                                                             (136, 1, 64, 64, 0), (24, 2, 64, 64, 0)])
-def test_prompt_portions(heads, kv_heads, dim, vdim, window, dtype):
+def test_prompt_portions(heads, kv_heads, dim, vdim, window, dtype, variant):
     """Whole prompts, portions behind a context, single tokens and a padding row among the tiles."""
-    run(spec(heads, kv_heads, dim, vdim, window), 128, [150, 70, 33, 1, 260, 64], [150, 31, 1, 1, 130, 64], dtype, heads + window, sink=heads == 8, tiles=True)
+    run(spec(heads, kv_heads, dim, vdim, window), 128, [150, 70, 33, 1, 260, 64], [150, 31, 1, 1, 130, 64], dtype, heads + window, sink=heads == 8, tiles=True, variant=variant)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [[100], [3, 1, 40]])
+def test_a_short_portion_behind_a_long_context(new, dtype):
+    """Few tiles: their keys are split."""
+    run(spec(8, 2, 128, 64), 64, [2500, 700, 1800][: len(new)], new, dtype, 5, sink=True, tiles=True)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -258,6 +268,10 @@ def test_large_and_small_magnitudes(variant, dtype):
         bt, seq, pos = torch.arange(1, 5, dtype=torch.int32).cuda()[None], torch.zeros(1, dtype=torch.long).cuda(), torch.tensor([n - 1]).cuda()
         want, big = attention(q, sp, seq, pos, held, None)
         close(ops.gqa_attention4(q, sp, cache, bt, seq, pos, None, None, variant), want, big, dtype)
+        many = q.expand(2, 90, 2, 64).contiguous()          # the same row in a tile of 90 tokens
+        t = torch.tensor([[0, 0, 64], [0, 64, 26]], dtype=torch.int32).cuda()
+        got = ops.gqa_attention4(many, sp, cache, bt, seq.expand(90).contiguous(), pos.expand(90).contiguous(), None, t, variant)
+        close(got, want.expand(90, -1), big, dtype, TALL)
 
 
 @pytest.mark.parametrize("variant", VARIANTS)
@@ -275,6 +289,7 @@ def test_what_is_not_a_number_stays_with_those_who_see_it(dtype, variant):
     bt = torch.arange(1, 4, dtype=torch.int32).cuda()[None]
     seq, pos = torch.zeros(n, dtype=torch.long).cuda(), torch.arange(n).cuda()
     t = torch.tensor([[0, i, min(64, n - i)] for i in range(0, n, 64)], dtype=torch.int32).cuda()
+    # two tiles of 64 and more rows, and single tokens
     for tiles in (None, t):
         out = ops.gqa_attention4(q, sp, cache, bt, seq, pos, None, tiles, variant).view(n, G, 2, 64).float().cpu()
         bad = torch.zeros(n, G, dtype=torch.bool)
@@ -385,5 +400,8 @@ def test_refusals():
                    dict(cache=cache.cpu()), dict(pos=slot.cpu())):
         with pytest.raises(ValueError):
             ops.gqa_attention4(**{**good, **change})
-    with pytest.raises(RuntimeError):
-        ops.gqa_attention4(**{**good, "variant": 9})
+    for variant in (9, -1):
+        with pytest.raises(RuntimeError):
+            ops.gqa_attention4(**{**good, "variant": variant})
+    with pytest.raises(RuntimeError):                       # no matrix instructions in 32 bits
+        ops.gqa_attention4(**{**good, "q": q.float(), "variant": 3})
