@@ -15,11 +15,13 @@
 // grows by more than 2^8 since the last time. Few tiles (decoding): the keys of a tile are split over blockIdx.y, and a
 // second kernel joins the parts.
 //
-// A 4-bit cache (FOUR; fl_cache4.cuh) has two more warps, which make the bf16 operands of a block in shared memory from its codes: a raw
+// A 4-bit cache (FOUR; fl_cache4.cuh) has two more warps, which make fp16 operands of a block in shared memory from its codes: a raw
 // block arrives by one bulk copy while the warps wait for a free stage, keys become K-major rows as a TMA copy would leave them,
-// values, whose codes lie along the tokens, a K-major V^T. Entries are exact in bf16, so everything behind the operands is the same
-// kernel. It is for tiles of many query rows, which share that work; short tiles have the kernel of fl_attention4.cuh, and each of
-// the two leaves the other's tiles alone.
+// values, whose codes lie along the tokens, a K-major V^T. An entry is its code times its scale times 2^(e - E), with E the largest
+// exponent of the block's keys (it goes into the scores), or of the values so far (the accumulator is rescaled when it grows): exact
+// for rows within 2^14 of the largest one, off by 2^-36 of that one's largest entry beyond. The queries are turned to fp16 in place,
+// each row times a power of two, and weights are held times 2^6. It is for tiles of many query rows, which share that work; short
+// tiles have the kernel of fl_attention4.cuh, and each of the two leaves the other's tiles alone.
 #pragma once
 
 #include "fl_attention4.cuh"
@@ -46,6 +48,10 @@ struct LatentShared {
   uint64_t full[LT_MAX_STAGES], empty[LT_MAX_STAGES], raw_full;
   uint64_t s_full[2], p_full[2], pv_done[2];
   float row_max[2][4][128], row_den[4][128];
+  // FOUR: the queries are fp16; the largest key exponent of a stage's block, the largest value exponent so far; of the query rows
+  uint64_t q_ready;
+  int exps[LT_MAX_STAGES][2];
+  short q_exp[128];
   uint32_t tmem_base, abort_flag;
 };
 
@@ -65,23 +71,20 @@ __host__ __device__ constexpr int lt_threads(int parts, bool four = false) { ret
 
 __device__ __forceinline__ void loaders_barrier() { asm volatile("bar.sync 9, %0;" ::"n"(32 * LT_LOADERS) : "memory"); }
 
-// fp16 products of a code and its scale (normal or zero) -> bf16, times the powers of two in `power`, 2^(112 + e): an fp16 number shifted
-// down by three bits is the bf16 of its 2^-112-fold. `high`: powers beyond that range, for the lanes that need them.
-__device__ __forceinline__ uint32_t bf16_of(uint32_t h, uint32_t power) {
-  const uint32_t t = (h >> 3 & 0x0fff0fffu) | (h & 0x80008000u);
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t), "r"(power));
-  return r;
+// A pair of fp16 scales times 2^-u, u in the halves of a word; deep: some u is beyond 14, where 2^-u is no normal fp16 any more.
+__device__ __forceinline__ uint32_t scaled_down(uint32_t scale, uint32_t u, bool deep) {
+  const uint32_t near = __vminu2(u, 0x000e000eu);
+  scale = hmul2(scale, (0x000f000fu - near) << 10);
+  if (deep) scale = hmul2(scale, (0x000f000fu - __vminu2(u - near, 0x000f000fu)) << 10);
+  return scale;
 }
-// 2^(112 + e) as bf16 in both halves from two exponent bytes e + 127 (in the low bytes of w's halves); up to e = 15.
-__device__ __forceinline__ uint32_t bf16_powers(uint32_t w) { return (w + 0x00700070u) << 7; }
 
 // One block's keys, by all loader threads: thread (row, column box) writes 64 entries of a row, 16 bytes at a time where a
-// 128-byte-swizzled copy would put them.
-__device__ __forceinline__ void operand_keys(const uint8_t* raw, uint8_t* st, const Cache4& c, int tid) {
+// 128-byte-swizzled copy would put them. deep: some row is more than 2^14 below E.
+__device__ __forceinline__ void operand_keys(const uint8_t* raw, uint8_t* st, const Cache4& c, int E, bool deep, int tid) {
   for (int u = tid; u < LT_KEYS * (c.K / 64); u += 32 * LT_LOADERS) {
-    const int r = u % LT_KEYS, box = u / LT_KEYS, e = raw[c.key_exp(r)];
-    const uint32_t finite = bf16_powers(min(e, 142) * 0x00010001u), more = (uint32_t)(e > 142 ? e - 142 + 127 : 127) * 0x00800080u;
+    const int r = u % LT_KEYS, box = u / LT_KEYS;
+    const uint32_t down = (E - min((int)raw[c.key_exp(r)], E)) * 0x00010001u;
     const uint4* codes = reinterpret_cast<const uint4*>(raw + r * (c.K / 2) + box * 32);
     uint8_t* row = st + box * (LT_KEYS * 128) + r * 128;
 #pragma unroll
@@ -89,23 +92,21 @@ __device__ __forceinline__ void operand_keys(const uint8_t* raw, uint8_t* st, co
       const uint4 v = codes[half];
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {                      // 8 codes: a chunk of 16 bytes
-        const uint32_t byte = raw[c.key_scale(r, box * 4 + half * 2 + k / 2)] & 127, scale = e4m3_pair(byte * 0x0101u);
-        const uint32_t power = byte == C4_NAN ? 0x7fff7fffu : finite;
-        uint32_t h[4];
-        e2m1_pairs(w[k], h);
+      for (int j = 0; j < 2; ++j) {                      // 16 codes: a scale, two chunks of 16 bytes
+        const uint32_t scale = scaled_down(e4m3_pair((raw[c.key_scale(r, box * 4 + half * 2 + j)] & 127) * 0x0101u), down, deep);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          h[x] = bf16_of(hmul2(h[x], scale), power);
-          if (e > 142) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(h[x]) : "r"(more));
+        for (int k = 2 * j; k < 2 * j + 2; ++k) {
+          uint32_t h[4];
+          e2m1_pairs(w[k], h);
+          *reinterpret_cast<uint4*>(row + (((half * 4 + k) ^ (r & 7)) << 4)) =
+              make_uint4(hmul2(h[0], scale), hmul2(h[1], scale), hmul2(h[2], scale), hmul2(h[3], scale));
         }
-        *reinterpret_cast<uint4*>(row + (((half * 4 + k) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
     }
   }
 }
 // Its values as V^T: thread (byte column, 16 tokens) writes two runs of 16 tokens, of entries 16 j + i and 16 j + i + 8.
-__device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, const Cache4& c, int tid) {
+__device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, const Cache4& c, int E, bool deep, int tid) {
   for (int u = tid; u < c.V / 2 * 4; u += 32 * LT_LOADERS) {
     const int col = u % (c.V / 2), t0 = u / (c.V / 2) * 16, j = col / 8, i = col % 8;
     const uint4 vc = *reinterpret_cast<const uint4*>(raw + 36 * c.K + col * C4_TOKENS + t0);
@@ -119,15 +120,10 @@ __device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, 
       e2m1_pairs(cw[q], h);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t scale = e4m3_pair(sw[q] >> (16 * x)), e = __byte_perm(ew[q], 0, x ? 0x4342 : 0x4140);
-        const uint32_t power = bf16_powers(__vminu2(e, 0x008e008eu));
-        lo[2 * q + x] = bf16_of(hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), scale), power);
-        hi[2 * q + x] = bf16_of(hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), scale), power);
-        if (__vmaxu2(e, 0x008e008eu) != 0x008e008eu) {
-          const uint32_t more = (__vmaxu2(e, 0x008e008eu) - 0x000f000fu) << 7;
-          asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(lo[2 * q + x]) : "r"(more));
-          asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(hi[2 * q + x]) : "r"(more));
-        }
+        const uint32_t most = (uint32_t)E * 0x00010001u, e = __vminu2(__byte_perm(ew[q], 0, x ? 0x4342 : 0x4140), most);
+        const uint32_t scale = scaled_down(e4m3_pair(sw[q] >> (16 * x)), most - e, deep);
+        lo[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), scale);
+        hi[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), scale);
       }
     }
     uint8_t* row = st + (16 * j + i) * 128;
@@ -138,6 +134,29 @@ __device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, 
       *reinterpret_cast<uint4*>(row + 8 * 128 + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
     }
   }
+}
+// A row of bf16 queries in its column boxes -> fp16 times 2^(14 - e), e the exponent of its largest magnitude (returned). Chunks are taken in an
+// order that spreads the rows of a warp over the banks.
+__device__ __forceinline__ int operand_query(uint8_t* qs, int q_box, int kcols, int r) {
+  float most = 0.0f;
+  for (int k = 0; k < kcols * 8; ++k) {
+    const uint4 v = *reinterpret_cast<const uint4*>(qs + (k / 8) * q_box + r * 128 + ((k + r) % 8) * 16);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
+  }
+  const int e = a4_query_exponent(most);
+  const float up = c4_power((A4_BIAS - e) / 2), up2 = c4_power(A4_BIAS - e - (A4_BIAS - e) / 2);
+  for (int k = 0; k < kcols * 8; ++k) {
+    uint4* at = reinterpret_cast<uint4*>(qs + (k / 8) * q_box + r * 128 + ((k + r) % 8) * 16);
+    uint32_t w[4] = {at->x, at->y, at->z, at->w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      w[x] = pack_half(__uint_as_float(w[x] << 16) * up * up2, __uint_as_float(w[x] & 0xffff0000u) * up * up2);
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return e;
 }
 
 // D (+)= A[tmem] * B[smem]; A: bf16 pairs, one row per lane.
@@ -210,6 +229,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       mbar_init(&sh->empty[i], 1);
     }
     mbar_init(&sh->raw_full, 1);
+    mbar_init(&sh->q_ready, LT_LOADERS);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], PARTS * quarters);
@@ -281,8 +301,9 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     if (lane == 0 && nb > 0) {
       // ---- MMA: scores of block i + 1 are issued before the values of block i. A query box of fewer than 128 rows is
       //      read on into what follows it in shared memory: those accumulator lanes belong to no query ----
-      constexpr uint32_t ID_S = umma_idesc_bf16(LT_KEYS);
-      const uint32_t id_v = umma_idesc_bf16((vn + 15) / 16 * 16, !FOUR);
+      constexpr uint32_t HALF = FOUR ? (1u << 7) | (1u << 10) : 0u;        // the operands' type bits: bf16 set, fp16 clear
+      constexpr uint32_t ID_S = umma_idesc_bf16(LT_KEYS) ^ HALF;
+      const uint32_t id_v = umma_idesc_bf16((vn + 15) / 16 * 16, !FOUR) ^ HALF;
       auto scores = [&](int i) {
         const int s = i % c.stages, buf = i & 1;
         if (!mbar_wait(&sh->full[s], (i / c.stages) & 1)) return false;
@@ -297,7 +318,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         umma_commit(&sh->s_full[buf]);
         return true;
       };
-      bool ok = mbar_wait(&sh->q_full, 0) && scores(0);
+      bool ok = mbar_wait(FOUR ? &sh->q_ready : &sh->q_full, 0) && scores(0);
       for (int i = 0; i < nb && ok; ++i) {
         const int s = i % c.stages, buf = i & 1;
         if (c.stages > 1 && i + 1 < nb && !(ok = scores(i + 1))) break;
@@ -329,7 +350,17 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     };
     if (nb > 0) fetch(0);
     // a wait that gives up is remembered and the loop goes on, without waits, copies or work: the barrier counts both warps
-    bool ok = true;
+    bool ok = nb == 0 || mbar_wait(&sh->q_full, 0);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && lane == 0) fail();
+    if (ok && nb > 0) {
+      for (int r = tid; r < c.qrows; r += 32 * LT_LOADERS) sh->q_exp[r] = (short)operand_query(qs, q_box, c.kcols, r);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->q_ready);
+    }
+    const int seen_lo = a.first_key(p_first);
+    int E = 0;                                           // the largest value exponent so far
     for (int i = 0; i < nb; ++i) {
       const int s = i % c.stages, round = i / c.stages;
       if (ok) {
@@ -338,9 +369,22 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         if (!ok && lane == 0) fail();
       }
       if (ok) {
+        // exponents of the tokens that some row of the tile sees
+        unsigned k_most = 0, v_most = 0, k_least = 255, v_least = 255;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t = lane + 32 * h;
+          const i64 key = (i64)(b0 + i) * LT_KEYS + t;
+          if (key < seen_lo || key > p_last) continue;
+          const unsigned ke = raw[c4.key_exp(t)], ve = raw[c4.value_exp(t)];
+          k_most = max(k_most, ke), v_most = max(v_most, ve), k_least = min(k_least, ke), v_least = min(v_least, ve);
+        }
+        k_most = __reduce_max_sync(0xffffffffu, k_most), k_least = __reduce_min_sync(0xffffffffu, k_least);
+        E = max(E, (int)__reduce_max_sync(0xffffffffu, v_most)), v_least = __reduce_min_sync(0xffffffffu, v_least);
         uint8_t* st = ring + s * stage_bytes;
-        operand_keys(raw, st, c4, tid);
-        operand_values(raw, st + c.kcols * LT_KEYS * 128, c4, tid);
+        operand_keys(raw, st, c4, (int)k_most, k_most > k_least + 14, tid);
+        operand_values(raw, st + c.kcols * LT_KEYS * 128, c4, E, E > (int)v_least + 14, tid);
+        if (tid == 0) sh->exps[s][0] = (int)k_most, sh->exps[s][1] = E;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->full[s]);
@@ -356,11 +400,21 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     const int flat = row0 + (live ? r : 0), token = tok0 + flat / a.H, head = group * a.H + flat % a.H;
     const i64 pos = min(a.pos[token], limit);
     const int lo = a.first_key(pos), hi = (int)pos;
-    const float scale = a.scale * LT_LOG2E;
+    constexpr float UNIT = FOUR ? 64.0f : 1.0f;          // what a weight of 1 is held as
+    constexpr float SHIFT = FOUR ? 6.0f : 0.0f;
+    float scale = a.scale * LT_LOG2E;
     float ref = a.sink ? a.sink[head] * LT_LOG2E : -INFINITY;
-    float den = a.sink && blockIdx.y == 0 && part == 0 ? 1.0f : 0.0f;
+    float den = a.sink && blockIdx.y == 0 && part == 0 ? UNIT : 0.0f;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
+    float row_scale = scale;
+    int E = 0;
+    if (FOUR && nb > 0) {
+      ok = mbar_wait(&sh->q_ready, 0);
+      __syncwarp();
+      const int back = ok ? sh->q_exp[r < c.qrows ? r : 0] - A4_BIAS : 0;
+      row_scale = scale * c4_power(back / 2) * c4_power(back - back / 2);
+    }
     for (int i = 0; i < nb; ++i) {
       const int buf = i & 1;
       ok = ok && mbar_wait(&sh->s_full[buf], (i >> 1) & 1);
@@ -370,6 +424,15 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
 #pragma unroll
       for (int k = 0; k < KW; k += 16) tmem_ld16(tmem + lanes + buf * LT_KEYS + part * KW + k, *reinterpret_cast<uint32_t(*)[16]>(u + k));
       tmem_ld_wait();
+      float f = 1.0f;
+      if (FOUR && ok) {
+        const int stage = i % c.stages;
+        ok = mbar_wait(&sh->full[stage], (i / c.stages) & 1);            // long done: orders the exponents
+        const int ek = sh->exps[stage][0], ev = sh->exps[stage][1];
+        scale = row_scale * c4_power(ek - 127);
+        if (ev != E && E != 0) f = c4_power(max(E - ev, -126));
+        E = ev;
+      }
       const int k0 = (b0 + i) * LT_KEYS + part * KW;
       float s[KW], mx = -INFINITY;
       if (k0 >= lo && k0 + KW - 1 <= hi) {
@@ -391,13 +454,14 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < PARTS; ++k) mx = fmaxf(mx, sh->row_max[buf][k][r]);
-      float f = 1.0f;
+      float g = 1.0f;
       if (mx > ref + LT_GROWTH || ref == -INFINITY) {
-        f = ref == -INFINITY ? 0.0f : exp2_fast(ref - mx);
+        g = ref == -INFINITY ? 0.0f : exp2_fast(ref - mx);
         ref = mx;
       }
+      den *= g;
+      f = FOUR ? f * g : g;
       if (__any_sync(0xffffffffu, f != 1.0f && live)) {    // the same in the four warps of the quarter
-        den *= f;
         if (i > 0) {
           // the accumulator may be touched once the values of block i - 1 are in
           ok = ok && mbar_wait(&sh->pv_done[buf ^ 1], ((i - 1) >> 1) & 1);
@@ -413,7 +477,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
           }
         }
       }
-      const float base = ref == -INFINITY ? 0.0f : ref;    // no visible key yet: every weight is 0
+      const float base = ref == -INFINITY ? 0.0f : ref - SHIFT;            // no visible key yet: every weight is 0
       float d0 = 0.0f, d1 = 0.0f;
       uint32_t w[KW / 2];
 #pragma unroll
@@ -421,7 +485,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         const float e0 = exp2_fast(s[2 * k] - base), e1 = exp2_fast(s[2 * k + 1] - base);
         d0 += e0;
         d1 += e1;
-        w[k] = pack_bf16(e0, e1);
+        w[k] = FOUR ? pack_half(e0, e1) : pack_bf16(e0, e1);
       }
       den += d0 + d1;
 #pragma unroll
@@ -444,7 +508,9 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     } else {
       tc_fence_after();
       const i64 n = (i64)a.M * a.H * a.G, at = (i64)token * a.H * a.G + head;
-      const float inv = 1.0f / den;
+      // outputs in units of 1: of the weights where a kernel behind joins parts
+      const float units = FOUR && E != 0 ? c4_power(max(E - 127, -126)) : 1.0f;
+      const float inv = c.splits == 1 ? units / den : units / UNIT;
       float* acc = c.part + (blockIdx.y * n + at) * a.R + v0;
       bf16* out = static_cast<bf16*>(a.out) + token * a.out_tok + head * a.out_head + v0;
       for (int q = part * 16; q < vn; q += 16 * PARTS) {
@@ -457,14 +523,14 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         const int cnt = min(16, vn - q);
         float v[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(u[k]) * (c.splits == 1 ? inv : 1.0f);
+        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(u[k]) * inv;
         if (c.splits == 1) store_run(out + q, v, cnt);
         else store_run(acc + q, v, cnt);
       }
       if (c.splits > 1 && live && v0 == 0 && part == 0) {
         float* ml = c.part + c.splits * n * a.R + (blockIdx.y * n + at) * 2;
         ml[0] = ref;
-        ml[1] = den;
+        ml[1] = den / UNIT;
       }
     }
   }
