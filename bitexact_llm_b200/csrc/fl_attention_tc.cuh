@@ -43,15 +43,19 @@ struct LatentTc {
   int min_rows;                                          // FOUR: tiles of fewer query rows are another kernel's
 };
 
+template <bool FOUR = false>
 struct LatentShared {
+  static constexpr int SHARE = FOUR ? 2 : 4;             // threads of a query row
+
   uint64_t q_full, o_done;
   uint64_t full[LT_MAX_STAGES], empty[LT_MAX_STAGES], raw_full;
   uint64_t s_full[2], p_full[2], pv_done[2];
-  float row_max[2][4][128], row_den[4][128];
+  float row_max[2][SHARE][128], row_den[SHARE][128];
   // FOUR: the queries are fp16; the largest key exponent of a stage's block, the largest value exponent so far; of the query rows
   uint64_t q_ready;
   int exps[LT_MAX_STAGES][2];
   short q_exp[128];
+  alignas(16) uint32_t scales[LT_VCOLS / 32 * LT_KEYS / 2];
   uint32_t tmem_base, abort_flag;
 };
 
@@ -80,58 +84,70 @@ __device__ __forceinline__ uint32_t scaled_down(uint32_t scale, uint32_t u, bool
 }
 
 // One block's keys, by all loader threads: thread (row, column box) writes 64 entries of a row, 16 bytes at a time where a
-// 128-byte-swizzled copy would put them. deep: some row is more than 2^14 below E.
-__device__ __forceinline__ void operand_keys(const uint8_t* raw, uint8_t* st, const Cache4& c, int E, bool deep, int tid) {
-  for (int u = tid; u < LT_KEYS * (c.K / 64); u += 32 * LT_LOADERS) {
-    const int r = u % LT_KEYS, box = u / LT_KEYS;
-    const uint32_t down = (E - min((int)raw[c.key_exp(r)], E)) * 0x00010001u;
+// 128-byte-swizzled copy would put them. deep: some row is more than 2^14 below E. What is read comes first: a load is not
+// moved in front of a store that might be to the same place.
+__device__ __forceinline__ void operand_keys(const uint8_t* __restrict__ raw, uint8_t* __restrict__ st, const Cache4& c, int E, bool deep, int tid) {
+  const int r = tid % LT_KEYS;
+  const uint32_t down = (E - min((int)raw[c.key_exp(r)], E)) * 0x00010001u;
+  for (int box = tid / LT_KEYS; box < c.K / 64; box += 32 * LT_LOADERS / LT_KEYS) {
     const uint4* codes = reinterpret_cast<const uint4*>(raw + r * (c.K / 2) + box * 32);
+    const uint4 v0 = codes[0], v1 = codes[1];
+    const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+    uint32_t scale[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) scale[j] = (raw[c.key_scale(r, box * 4 + j)] & 127) * 0x0101u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) scale[j] = scaled_down(e4m3_pair(scale[j]), down, deep);
     uint8_t* row = st + box * (LT_KEYS * 128) + r * 128;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint4 v = codes[half];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {                      // 16 codes: a scale, two chunks of 16 bytes
-        const uint32_t scale = scaled_down(e4m3_pair((raw[c.key_scale(r, box * 4 + half * 2 + j)] & 127) * 0x0101u), down, deep);
-#pragma unroll
-        for (int k = 2 * j; k < 2 * j + 2; ++k) {
-          uint32_t h[4];
-          e2m1_pairs(w[k], h);
-          *reinterpret_cast<uint4*>(row + (((half * 4 + k) ^ (r & 7)) << 4)) =
-              make_uint4(hmul2(h[0], scale), hmul2(h[1], scale), hmul2(h[2], scale), hmul2(h[3], scale));
-        }
-      }
+    for (int k = 0; k < 8; ++k) {
+      uint32_t h[4];
+      e2m1_pairs(w[k], h);
+      *reinterpret_cast<uint4*>(row + ((k ^ (r & 7)) << 4)) =
+          make_uint4(hmul2(h[0], scale[k / 2]), hmul2(h[1], scale[k / 2]), hmul2(h[2], scale[k / 2]), hmul2(h[3], scale[k / 2]));
     }
   }
 }
+// Scales of its values as fp16 pairs of tokens relative to E: word (j, pair) for entries 16 j .. 16 j + 15.
+__device__ __forceinline__ void operand_scales(const uint8_t* __restrict__ raw, uint32_t* __restrict__ scales, const Cache4& c, int E, bool deep,
+                                               int tid) {
+  const uint32_t most = (uint32_t)E * 0x00010001u;
+  for (int u = tid; u < c.V / 16 * (LT_KEYS / 4); u += 32 * LT_LOADERS) {                 // four tokens
+    const int j = u / (LT_KEYS / 4), t = u % (LT_KEYS / 4) * 4;
+    const uint32_t s = *reinterpret_cast<const uint32_t*>(raw + 36 * c.K + 32 * c.V + j * C4_TOKENS + t);
+    const uint32_t e = *reinterpret_cast<const uint32_t*>(raw + 36 * (c.K + c.V) + C4_TOKENS + t);
+    const uint32_t lo = scaled_down(e4m3_pair(s), most - __vminu2(__byte_perm(e, 0, 0x4140), most), deep);
+    const uint32_t hi = scaled_down(e4m3_pair(s >> 16), most - __vminu2(__byte_perm(e, 0, 0x4342), most), deep);
+    *reinterpret_cast<uint2*>(scales + j * (LT_KEYS / 2) + t / 2) = make_uint2(lo, hi);
+  }
+}
 // Its values as V^T: thread (byte column, 16 tokens) writes two runs of 16 tokens, of entries 16 j + i and 16 j + i + 8.
-__device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, const Cache4& c, int E, bool deep, int tid) {
-  for (int u = tid; u < c.V / 2 * 4; u += 32 * LT_LOADERS) {
-    const int col = u % (c.V / 2), t0 = u / (c.V / 2) * 16, j = col / 8, i = col % 8;
+__device__ __forceinline__ void operand_values(const uint8_t* __restrict__ raw, const uint32_t* __restrict__ scales, uint8_t* __restrict__ st,
+                                               const Cache4& c, int tid) {
+  const int columns = c.V / 2;                           // 32 or 64
+#pragma unroll 2
+  for (int u = tid; u < columns * 4; u += 32 * LT_LOADERS) {
+    const int col = u & (columns - 1), t0 = u / columns * 16, j = col / 8, i = col % 8;
     const uint4 vc = *reinterpret_cast<const uint4*>(raw + 36 * c.K + col * C4_TOKENS + t0);
-    const uint4 vs = *reinterpret_cast<const uint4*>(raw + 36 * c.K + 32 * c.V + j * C4_TOKENS + t0);
-    const uint4 ve = *reinterpret_cast<const uint4*>(raw + 36 * (c.K + c.V) + C4_TOKENS + t0);
-    const uint32_t cw[4] = {vc.x, vc.y, vc.z, vc.w}, sw[4] = {vs.x, vs.y, vs.z, vs.w}, ew[4] = {ve.x, ve.y, ve.z, ve.w};
-    uint32_t lo[8], hi[8];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {                        // 4 tokens
-      uint32_t h[4];
-      e2m1_pairs(cw[q], h);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint32_t most = (uint32_t)E * 0x00010001u, e = __vminu2(__byte_perm(ew[q], 0, x ? 0x4342 : 0x4140), most);
-        const uint32_t scale = scaled_down(e4m3_pair(sw[q] >> (16 * x)), most - e, deep);
-        lo[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), scale);
-        hi[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), scale);
-      }
-    }
+    const uint4 s0 = *reinterpret_cast<const uint4*>(scales + j * (LT_KEYS / 2) + t0 / 2), s1 = *reinterpret_cast<const uint4*>(scales + j * (LT_KEYS / 2) + t0 / 2 + 4);
+    const uint32_t cw[4] = {vc.x, vc.y, vc.z, vc.w}, sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
     uint8_t* row = st + (16 * j + i) * 128;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 2; ++k) {                        // 8 tokens: a chunk of 16 bytes for each of the two entries
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t h[4];
+        e2m1_pairs(cw[2 * k + q], h);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          lo[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), sw[4 * k + 2 * q + x]);
+          hi[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), sw[4 * k + 2 * q + x]);
+        }
+      }
       const int at = (t0 / 8 + k ^ i) << 4;              // 16 j + i and + 8 are alike modulo 8
-      *reinterpret_cast<uint4*>(row + at) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
-      *reinterpret_cast<uint4*>(row + 8 * 128 + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+      *reinterpret_cast<uint4*>(row + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      *reinterpret_cast<uint4*>(row + 8 * 128 + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     }
   }
 }
@@ -139,22 +155,32 @@ __device__ __forceinline__ void operand_values(const uint8_t* raw, uint8_t* st, 
 // order that spreads the rows of a warp over the banks.
 __device__ __forceinline__ int operand_query(uint8_t* qs, int q_box, int kcols, int r) {
   float most = 0.0f;
-  for (int k = 0; k < kcols * 8; ++k) {
-    const uint4 v = *reinterpret_cast<const uint4*>(qs + (k / 8) * q_box + r * 128 + ((k + r) % 8) * 16);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int box = 0; box < kcols; ++box) {
+    const uint8_t* row = qs + box * q_box + r * 128;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
+    for (int k = 0; k < 8; ++k) {
+      const uint4 v = *reinterpret_cast<const uint4*>(row + (((k + r) & 7) << 4));
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
+    }
   }
   const int e = a4_query_exponent(most);
   const float up = c4_power((A4_BIAS - e) / 2), up2 = c4_power(A4_BIAS - e - (A4_BIAS - e) / 2);
-  for (int k = 0; k < kcols * 8; ++k) {
-    uint4* at = reinterpret_cast<uint4*>(qs + (k / 8) * q_box + r * 128 + ((k + r) % 8) * 16);
-    uint32_t w[4] = {at->x, at->y, at->z, at->w};
+  for (int box = 0; box < kcols; ++box) {
+    uint8_t* row = qs + box * q_box + r * 128;
+    uint4 v[8];
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      w[x] = pack_half(__uint_as_float(w[x] << 16) * up * up2, __uint_as_float(w[x] & 0xffff0000u) * up * up2);
-    *at = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4*>(row + (((k + r) & 7) << 4));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        w[x] = pack_half(__uint_as_float(w[x] << 16) * up * up2, __uint_as_float(w[x] & 0xffff0000u) * up * up2);
+      *reinterpret_cast<uint4*>(row + (((k + r) & 7) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
   return e;
 }
@@ -190,8 +216,10 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
   const int q_box = c.qrows * 128;                       // bytes of a column block of the queries
   uint8_t* ring = qs + c.kcols * q_box;
   const int stage_bytes = c.cols * LT_KEYS * 128;
-  LatentShared* sh = reinterpret_cast<LatentShared*>(ring + c.stages * stage_bytes);
-  uint8_t* raw = reinterpret_cast<uint8_t*>(sh) + (sizeof(LatentShared) + 15) / 16 * 16;           // FOUR: a block as it is in the cache
+  using Shared = LatentShared<FOUR>;
+  static_assert(PARTS <= Shared::SHARE, "threads of a row");
+  Shared* sh = reinterpret_cast<Shared*>(ring + c.stages * stage_bytes);
+  uint8_t* raw = reinterpret_cast<uint8_t*>(sh) + (sizeof(Shared) + 15) / 16 * 16;           // FOUR: a block as it is in the cache
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   wait_previous();
@@ -200,7 +228,8 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
   int tok0, ntok;
   i64 seq;
   if (a.tiles) {
-    const int* t = a.tiles + (i64)blockIdx.x * 3;
+    // (FOUR: from the end, where the long contexts of a prompt are, so that the last tiles to be done are short ones)
+    const int* t = a.tiles + (i64)(FOUR ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * 3;
     seq = t[0];
     tok0 = t[1];
     ntok = t[2];
@@ -382,9 +411,13 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         k_most = __reduce_max_sync(0xffffffffu, k_most), k_least = __reduce_min_sync(0xffffffffu, k_least);
         E = max(E, (int)__reduce_max_sync(0xffffffffu, v_most)), v_least = __reduce_min_sync(0xffffffffu, v_least);
         uint8_t* st = ring + s * stage_bytes;
+        operand_scales(raw, sh->scales, c4, E, E > (int)v_least + 14, tid);
         operand_keys(raw, st, c4, (int)k_most, k_most > k_least + 14, tid);
-        operand_values(raw, st + c.kcols * LT_KEYS * 128, c4, E, E > (int)v_least + 14, tid);
         if (tid == 0) sh->exps[s][0] = (int)k_most, sh->exps[s][1] = E;
+      }
+      loaders_barrier();                                 // the scales are there
+      if (ok) {
+        operand_values(raw, sh->scales, ring + s * stage_bytes + c.kcols * LT_KEYS * 128, c4, tid);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->full[s]);

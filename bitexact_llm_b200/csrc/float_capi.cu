@@ -229,7 +229,7 @@ constexpr int LT_PAIR_SMEM = 113 * 1024;
 bool paged_pair_fits(const PagedAttn& a) {
   const int kcols = ceil_div(a.W, 64), cols = kcols + (a.voff > 0 ? ceil_div(a.R, 64) : 0);
   const int rows = (a.tiles ? bxf_latent_attention_tile(a.H) : 1) * a.H, qrows = rows >= 128 ? 128 : ceil_div(rows, 8) * 8;
-  return a.R <= 128 && 1024 + kcols * qrows * 128 + (int)sizeof(LatentShared) + 2 * cols * LT_KEYS * 128 <= LT_PAIR_SMEM;
+  return a.R <= 128 && 1024 + kcols * qrows * 128 + (int)sizeof(LatentShared<>) + 2 * cols * LT_KEYS * 128 <= LT_PAIR_SMEM;
 }
 
 size_t attention_scratch(i64 rows, int R, int splits) { return (size_t)splits * rows * (R + 2) * sizeof(float); }
@@ -256,7 +256,7 @@ int launch_paged_tc(const PagedAttn& a, void* scratch, size_t scratch_bytes, cud
   const int tokens = a.tiles ? bxf_latent_attention_tile(a.H) : 1, tiles = a.tiles ? a.ntiles : a.M;
   const int rows = tokens * a.H;
   c.qrows = rows >= 128 ? 128 : ceil_div(rows, 8) * 8;
-  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared);
+  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared<>);
   c.stages = (SMEM_MAX - fixed) / (c.cols * LT_KEYS * 128);
   if (c.stages > LT_MAX_STAGES) c.stages = LT_MAX_STAGES;
   c.row_blocks = ceil_div(rows, 128);
@@ -360,7 +360,7 @@ int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, voi
   c.min_rows = min_rows;
   const int tokens = bxf_latent_attention_tile(a.H), rows = tokens * a.H;
   c.qrows = rows >= 128 ? 128 : ceil_div(rows, 8) * 8;
-  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared) + 16 + c4.bytes();
+  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared<true>) + 16 + c4.bytes();
   c.stages = (LT_PAIR_SMEM - fixed) / (c.cols * LT_KEYS * 128);
   if (c.stages > LT_MAX_STAGES) c.stages = LT_MAX_STAGES;
   c.row_blocks = ceil_div(rows, 128);
