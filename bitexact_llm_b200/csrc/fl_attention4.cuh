@@ -100,15 +100,17 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
 //            values so far: like the running maximum, the accumulators follow it when it grows
 // A transposed 8x8 register exchange (movmatrix) turns P into the second product's operand: nothing goes through shared memory but the blocks.
 //
-// A warp takes every fourth block of its CTA's keys, in a ring of its own filled by bulk copies (one per block): warps never wait for one
-// another until the end. A tile's keys are cut over a cluster of CTAs when there are few tiles; the parts are joined through distributed shared
-// memory in a fixed order, so there is one launch, no scratch memory, and the same bits in every call.
-constexpr int A4_WARPS = 4, A4_STAGES = 2, A4_MAX_CLUSTER = 16, A4_ROWS_MAX = 16;
+// A tile belongs to one warp (CTAs of one: many tiles), to the W = 4 warps of a CTA, or to a cluster of those (few tiles). A warp takes every
+// W-th block of its CTA's keys, in a ring of its own filled by bulk copies (one per block): warps never wait for one another until
+// the end. The parts are joined through shared memory and that of the cluster in a fixed order, so there is one launch, no scratch
+// memory, and the same bits in every call.
+constexpr int A4_STAGES = 2, A4_MAX_CLUSTER = 16, A4_ROWS_MAX = 16;
 constexpr int A4_BIAS = 14;            // weights are kept times 2^14
 
+template <int W>
 struct A4Shared {
-  uint64_t full[A4_WARPS][A4_STAGES];
-  float max_[A4_WARPS][A4_ROWS_MAX], den[A4_WARPS][A4_ROWS_MAX];         // per warp and row
+  uint64_t full[W][A4_STAGES];
+  float max_[W][A4_ROWS_MAX], den[W][A4_ROWS_MAX];                       // per warp and row
   float row_max[A4_ROWS_MAX], row_den[A4_ROWS_MAX];                      // of the CTA
   uint32_t abort_flag;
 };
@@ -176,34 +178,35 @@ __device__ __forceinline__ int a4_query_exponent(float most) {
 template <int K, int V>
 __host__ __device__ constexpr int a4_block_bytes() { return 36 * (K + V) + 2 * C4_TOKENS; }
 // The warps' rings; at the end the same memory holds the warps' outputs, rows of V floats.
-template <int K, int V, int NT>
+template <int K, int V, int NT, int W>
 __host__ __device__ constexpr int a4_ring_bytes() {
-  const int ring = A4_WARPS * A4_STAGES * a4_block_bytes<K, V>(), out = (A4_WARPS + 1) * 8 * NT * V * 4;
+  const int ring = W * A4_STAGES * a4_block_bytes<K, V>(), out = (W > 1 ? W + 1 : 1) * 8 * NT * V * 4;
   return ring > out ? ring : out;
 }
 
-template <int K, int V, int NT>
-__global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_kernel(const PagedAttn a, const Cache4 c, int max_rows) {
+template <int K, int V, int NT, int W>
+__global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_kernel(const PagedAttn a, const Cache4 c, int max_rows) {
   constexpr int BYTES = a4_block_bytes<K, V>(), KS = K / 16, KW = K / 32, ROWS = 8 * NT;
   extern __shared__ __align__(128) uint8_t a4_raw[];
   uint8_t* ring_all = a4_raw;
-  A4Shared* sh = reinterpret_cast<A4Shared*>(a4_raw + a4_ring_bytes<K, V, NT>());
+  auto* sh = reinterpret_cast<A4Shared<W>*>(a4_raw + a4_ring_bytes<K, V, NT, W>());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   uint32_t rank, ctas;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
   if (threadIdx.x == 0) {
-    for (int w = 0; w < A4_WARPS; ++w)
+    for (int w = 0; w < W; ++w)
       for (int s = 0; s < A4_STAGES; ++s) mbar_init(&sh->full[w][s], 1);
     sh->abort_flag = *reinterpret_cast<volatile int*>(&g_wait_timeouts) != 0;
     fence_barrier_init();
   }
-  __syncthreads();
+  if constexpr (W > 1) __syncthreads();
+  else __syncwarp();
   launch_next();
   wait_previous();
 
   // ---- the tile ----
-  const int tile = blockIdx.x / ctas, group = blockIdx.y;
+  const int tile = blockIdx.x >> (__ffs(ctas) - 1), group = blockIdx.y;
   int tok0, ntok;
   i64 seq;
   if (a.tiles) {
@@ -216,41 +219,14 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
   const int row0 = blockIdx.z * ROWS, rows = min(ROWS, ntok * a.H - row0);
   if (rows <= 0 || a.tiles && ntok * a.H > max_rows) return;             // all CTAs of the cluster alike; taller tiles are another kernel's
   const i64 limit = (i64)a.nblk * a.bs - 1;
-  const int t_first = row0 / a.H, t_last = (row0 + rows - 1) / a.H;
-  const i64 p_first = min(a.pos[tok0 + t_first], limit), p_last = min(a.pos[tok0 + t_last], limit);
-  const int lo_all = a.first_key(p_first), b_lo = lo_all / C4_TOKENS, b_hi = p_last < 0 ? b_lo : (int)(p_last / C4_TOKENS) + 1;
-  const int b0 = b_lo + (int)((i64)(b_hi - b_lo) * rank / ctas), b1 = b_lo + (int)((i64)(b_hi - b_lo) * (rank + 1) / ctas);
-  const int n = b1 - b0 > warp ? (b1 - b0 - warp + A4_WARPS - 1) / A4_WARPS : 0;          // the warp's blocks: b0 + warp + 4 i
-  uint8_t* ring = ring_all + warp * A4_STAGES * BYTES;
-  bool ok = sh->abort_flag == 0;
-
-  int held = 0;
-  auto fetch = [&](int i) {                                // block i of the warp; the warp reads the block table for 32 blocks at a time
-    if ((i & 31) == 0) {
-      const int b = min(b0 + warp + (i + lane) * A4_WARPS, b_hi - 1);
-      held = (int)a.page_of(seq, min(b * C4_TOKENS / a.bs, a.nblk - 1));
-    }
-    const i64 page = __shfl_sync(0xffffffffu, held, i & 31);
-    if (lane == 0) {
-      const int in_page = (b0 + warp + i * A4_WARPS) % (a.bs / C4_TOKENS);
-      uint64_t* bar = &sh->full[warp][i % A4_STAGES];
-      mbar_arrive_expect_tx(bar, BYTES);
-      bulk_load(ring + i % A4_STAGES * BYTES, c.p + ((page * a.G + group) * (a.bs / C4_TOKENS) + in_page) * BYTES, bar, BYTES);
-    }
-  };
-  if (ok)
-    for (int i = 0; i < A4_STAGES && i < n; ++i) fetch(i);
-
-  // ---- queries: thread (gid, tig) holds, of row gid of every group of 8, entries tig K / 4 .. ----
+  // what depends on nothing but the tile is asked for ahead of the chain position, page, block
   uint32_t q[NT][KS][2];
-  float row_scale[NT][2];                                  // of rows 2 tig, 2 tig + 1: what a score is worth in powers of two
-  int row_lo[NT][2], row_hi[NT][2];
+  i64 row_pos[NT][2];                                      // of rows 2 tig, 2 tig + 1
   const bool wide = a.ldq % 4 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int flat = row0 + min(8 * t + gid, rows - 1);
     const bf16* from = static_cast<const bf16*>(a.q) + (((i64)group * a.M + tok0 + flat / a.H) * a.H + flat % a.H) * a.ldq + tig * (K / 4);
-    float most = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int d = tig * (K / 4) + 4 * s;
@@ -264,10 +240,46 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
         q[t][s][0] = pack_bf16(v[0], v[1]);
         q[t][s][1] = pack_bf16(v[2], v[3]);
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) row_pos[t][h] = a.pos[tok0 + (row0 + min(8 * t + 2 * tig + h, rows - 1)) / a.H];
+  }
+  const int t_first = row0 / a.H, t_last = (row0 + rows - 1) / a.H;
+  const i64 p_first = min(a.pos[tok0 + t_first], limit), p_last = min(a.pos[tok0 + t_last], limit);
+  const int lo_all = a.first_key(p_first), b_lo = lo_all / C4_TOKENS, b_hi = p_last < 0 ? b_lo : (int)(p_last / C4_TOKENS) + 1;
+  const int b0 = b_lo + (int)((i64)(b_hi - b_lo) * rank / ctas), b1 = b_lo + (int)((i64)(b_hi - b_lo) * (rank + 1) / ctas);
+  const int n = b1 - b0 > warp ? (b1 - b0 - warp + W - 1) / W : 0;          // the warp's blocks: b0 + warp + 4 i
+  uint8_t* ring = ring_all + warp * A4_STAGES * BYTES;
+  bool ok = sh->abort_flag == 0;
+
+  int held = 0;
+  auto fetch = [&](int i) {                                // block i of the warp; the warp reads the block table for 32 blocks at a time
+    if ((i & 31) == 0) {
+      const int b = min(b0 + warp + (i + lane) * W, b_hi - 1);
+      held = (int)a.page_of(seq, min(b * C4_TOKENS / a.bs, a.nblk - 1));
+    }
+    const i64 page = __shfl_sync(0xffffffffu, held, i & 31);
+    if (lane == 0) {
+      const int in_page = (b0 + warp + i * W) % (a.bs / C4_TOKENS);
+      uint64_t* bar = &sh->full[warp][i % A4_STAGES];
+      mbar_arrive_expect_tx(bar, BYTES);
+      bulk_load(ring + i % A4_STAGES * BYTES, c.p + ((page * a.G + group) * (a.bs / C4_TOKENS) + in_page) * BYTES, bar, BYTES);
+    }
+  };
+  if (ok)
+    for (int i = 0; i < A4_STAGES && i < n; ++i) fetch(i);
+
+  // ---- queries: thread (gid, tig) holds, of row gid of every group of 8, entries tig K / 4 .. ----
+  float row_scale[NT][2];                                  // of rows 2 tig, 2 tig + 1: what a score is worth in powers of two
+  int row_lo[NT][2], row_hi[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         most = fmaxf(most, fmaxf(fabsf(__uint_as_float(q[t][s][h] << 16)), fabsf(__uint_as_float(q[t][s][h] & 0xffff0000u))));
-    }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     const int e = a4_query_exponent(most);
@@ -282,8 +294,7 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
     for (int h = 0; h < 2; ++h) {
       const int back = __shfl_sync(0xffffffffu, e, (2 * tig + h) * 4) - A4_BIAS;
       row_scale[t][h] = a.scale * 1.4426950408889634f * c4_power(back / 2) * c4_power(back - back / 2);
-      const int f = row0 + min(8 * t + 2 * tig + h, rows - 1);
-      const i64 p = min(a.pos[tok0 + f / a.H], limit);
+      const i64 p = min(row_pos[t][h], limit);
       row_lo[t][h] = a.first_key(p);
       row_hi[t][h] = (int)p;
     }
@@ -311,7 +322,7 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
       break;
     }
     const uint8_t* blk = ring + i % A4_STAGES * BYTES;
-    const int k0 = (b0 + warp + i * A4_WARPS) * C4_TOKENS;
+    const int k0 = (b0 + warp + i * W) * C4_TOKENS;
 
     // ---- scores: m-tile u holds tokens 16 (gid / 2) + 4 u + gid % 2 in its rows gid, and those + 2 in rows gid + 8 ----
     float s[4][NT][4] = {};
@@ -453,6 +464,10 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
   }
 
   // ---- the CTA's part: rows of V outputs per warp, in units of 1 ----
+  auto together = [] {
+    if constexpr (W > 1) __syncthreads();
+    else __syncwarp();
+  };
   if (!ok) sh->abort_flag = 1;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -462,9 +477,9 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
       for (int o = 4; o < 32; o <<= 1) den[t][h] += __shfl_xor_sync(0xffffffffu, den[t][h], o);
       if (gid == 0) sh->max_[warp][8 * t + 2 * tig + h] = top[t][h], sh->den[warp][8 * t + 2 * tig + h] = den[t][h];
     }
-  __syncthreads();                                         // all rings are done with
+  together();                                              // all rings are done with
   const bool dead = sh->abort_flag != 0;
-  float* slab = reinterpret_cast<float*>(ring_all);        // [row][V] of the CTA, then of every warp
+  float* slab = reinterpret_cast<float*>(ring_all);        // [row][V] of the CTA, then (W > 1) of every warp
   const float unit = E == 0 ? 0.0f : c4_power(max(E - 127 - A4_BIAS, -126));
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -473,49 +488,76 @@ __global__ void __launch_bounds__(32 * A4_WARPS, NT == 1 ? 3 : 2) fl_attention4_
       const int r = 8 * t + 2 * tig + h;
       float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < A4_WARPS; ++w) m = fmaxf(m, sh->max_[w][r]);
+      for (int w = 0; w < W; ++w) m = fmaxf(m, sh->max_[w][r]);
       const float g = unit * (top[t][h] == -INFINITY ? 0.0f : a4_exp2(top[t][h] - m));
+      float* to = slab + ((W > 1 ? warp + 1 : 0) * ROWS + r) * V + gid;
 #pragma unroll
       for (int j = 0; j < V / 16; ++j) {
-        slab[((warp + 1) * ROWS + r) * V + 16 * j + gid] = out[j][t][h] * g;
-        slab[((warp + 1) * ROWS + r) * V + 16 * j + gid + 8] = out[j][t][h + 2] * g;
+        to[16 * j] = out[j][t][h] * g;
+        to[16 * j + 8] = out[j][t][h + 2] * g;
       }
       if (warp == 0 && gid == 0) {
         float d = 0.0f;
 #pragma unroll
-        for (int w = 0; w < A4_WARPS; ++w) d += sh->max_[w][r] == -INFINITY ? sh->den[w][r] : sh->den[w][r] * a4_exp2(sh->max_[w][r] - m);
+        for (int w = 0; w < W; ++w) d += sh->max_[w][r] == -INFINITY ? sh->den[w][r] : sh->den[w][r] * a4_exp2(sh->max_[w][r] - m);
         sh->row_max[r] = m;
         sh->row_den[r] = d;
       }
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < ROWS * V; i += 32 * A4_WARPS) {
-    float v = 0.0f;
+  together();
+  if constexpr (W > 1) {
+    for (int i = threadIdx.x; i < ROWS * V; i += 32 * W) {
+      float v = 0.0f;
 #pragma unroll
-    for (int w = 1; w <= A4_WARPS; ++w) v += slab[w * ROWS * V + i];
-    slab[i] = v;
+      for (int w = 1; w <= W; ++w) v += slab[w * ROWS * V + i];
+      slab[i] = v;
+    }
+    __syncthreads();
   }
-  cluster_arrive();
-  cluster_wait();
-  // ---- the row: every CTA of the cluster finishes a part of the outputs ----
-  if (!dead) {
-    const uint32_t slab_at = smem_u32(slab), max_at = smem_u32(sh->row_max), den_at = smem_u32(sh->row_den);
-    for (int i = rank * 32 * A4_WARPS + threadIdx.x; i < rows * V; i += ctas * 32 * A4_WARPS) {
-      const int r = i / V, d = i % V, flat = row0 + r, head = group * a.H + flat % a.H;
-      if (d >= a.R) continue;
-      float m = a.sink ? a.sink[head] * 1.4426950408889634f : -INFINITY, sum = 0.0f, v = 0.0f;
-      const float sink = m;
+  // ---- the rows: every CTA of the cluster finishes a part of the outputs, a thread four entries ----
+  const bool quads = a.R % 4 == 0 && a.out_tok % 4 == 0 && a.out_head % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
+  if (ctas > 1) {
+    cluster_arrive();
+    cluster_wait();
+  } else if (dead) {
+    return;
+  }
+  const uint32_t slab_at = smem_u32(slab), max_at = smem_u32(sh->row_max), den_at = smem_u32(sh->row_den);
+  for (int i = (rank * 32 * W + threadIdx.x) * 4; i < rows * V && !dead; i += ctas * 32 * W * 4) {
+    const int r = i / V, d = i % V, flat = row0 + r, head = group * a.H + flat % a.H;
+    if (d >= a.R) continue;
+    const float sink = a.sink ? a.sink[head] * 1.4426950408889634f : -INFINITY;
+    float m = sink, sum = 0.0f, v[4] = {};
+    if (ctas == 1) {
+      const float mk = sh->row_max[r], dk = sh->row_den[r];
+      m = fmaxf(m, mk);
+      const float g = mk == -INFINITY ? (dk == 0.0f ? 0.0f : 1.0f) : a4_exp2(mk - m);      // a part with no key has no weight
+      sum = g * dk;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = g * slab[i + e];
+    } else {
       for (uint32_t k = 0; k < ctas; ++k) m = fmaxf(m, ld_cluster(mapa_shared(max_at + 4 * r, k)));
-      if (a.sink) sum = a4_exp2(sink - m);
       for (uint32_t k = 0; k < ctas; ++k) {
         const float mk = ld_cluster(mapa_shared(max_at + 4 * r, k)), dk = ld_cluster(mapa_shared(den_at + 4 * r, k));
-        const float g = mk == -INFINITY ? (dk == 0.0f ? 0.0f : 1.0f) : a4_exp2(mk - m);      // a part with no key has no weight
+        const float g = mk == -INFINITY ? (dk == 0.0f ? 0.0f : 1.0f) : a4_exp2(mk - m);
+        const uint32_t from = mapa_shared(slab_at + 4 * i, k);
         sum += g * dk;
-        v += g * ld_cluster(mapa_shared(slab_at + 4 * i, k));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += g * ld_cluster(from + 4 * e);
       }
-      st(static_cast<bf16*>(a.out) + (tok0 + flat / a.H) * a.out_tok + head * a.out_head + d, sum == 0.0f ? 0.0f : v / sum);
+    }
+    if (a.sink) sum += a4_exp2(sink - m);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    bf16* to = static_cast<bf16*>(a.out) + (tok0 + flat / a.H) * a.out_tok + head * a.out_head + d;
+    if (quads) {
+      st4(to, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < a.R) st(to + e, v[e] * inv);
     }
   }
+  if (ctas == 1) return;
   cluster_arrive();                                        // nobody leaves while its memory may be read
   cluster_wait();
 }

@@ -319,26 +319,49 @@ int launch_store4(const Store4<T>& a, cudaStream_t st) {
 
 bool attention4_fits(int dtype, const Cache4& c) { return dtype == BXF_BF16 && c.K <= 128 && c.V <= 128; }
 
-// CTAs that share the keys of a tile: a power of two, until the SMs have their three CTAs, as long as every warp has a block to work on.
-int attention4_cluster(i64 tiles, i64 blocks, int per_sm) {
+// How the keys of a tile are shared: CTAs of one warp or of four, and CTAs per tile (a power of two). The contexts are on the device:
+// they are taken to fill the block table. Measured (us; 8 key/value heads, 1 / 2 / 4 / 8 / 16 CTAs of four warps a tile, one warp):
+//   1 x 2000 keys of 128 entries       16.9  12.4   9.2   8.0   9.0,  52    steps of a warp: 8 .. 0.5
+//   4 x 300 .. 3000                    22.6  15.3  13.2  11.7  18.4,  74
+//   32 x 100 .. 4000                   50.8  36.4  39.7  58.2   114,  98    CTAs: 256, 512, .. on 444 places
+//   64 x 8192                           153   138   158   199   309, 293    512 (two rounds), 1024 (three), ..
+//   16 x 8000, 64 entries              62.4  43.8  28.1  33.4  47.5, 133    128, 256, 512 on 592 places, ..
+//   600 x 100 .. 300, 64 entries       53.5                          45.7
+// So: as many CTAs as there are places (a quarter more does no harm), while every warp has a block; twice that where a second
+// round would be mostly empty and parts stay long; one warp a tile where there is hardly a block for each of four.
+struct Share4 {
+  int warps, ctas;
+};
+Share4 attention4_share(i64 tiles, i64 blocks, int per_sm) {
+  const i64 places = (i64)per_sm * device_sms();
+  if (blocks <= 6 && tiles >= 4 * places) return {1, 1};
   int c = 1;
-  while (c < A4_MAX_CLUSTER && tiles * c * 2 <= (i64)per_sm * device_sms() && blocks >= 2 * c * A4_WARPS) c *= 2;
-  return c;
+  while (c < A4_MAX_CLUSTER && tiles * c * 2 * 4 <= places * 5 && blocks >= 8 * c) c *= 2;
+  const i64 ctas = tiles * c, rounds = (ctas + places - 1) / places;
+  if (rounds > 1 && 10 * rounds * places > 13 * ctas && c < A4_MAX_CLUSTER && blocks >= 64 * c) c *= 2;
+  return {4, c};
+}
+
+template <int K, int V, int NT, int W>
+int launch_attention4(const PagedAttn& a, const Cache4& c, int most, dim3 grid, int cluster, cudaStream_t st) {
+  constexpr int smem = a4_ring_bytes<K, V, NT, W>() + sizeof(A4Shared<W>);
+  static PerDevice configured;
+  if (once_per_device(configured, [] {
+        const cudaError_t e = cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      }) != BX_OK)
+    return BX_ELAUNCH;
+  return launch_chained(fl_attention4_kernel<K, V, NT, W>, grid, 32 * W, smem, st, cluster, a, c, most);
 }
 
 template <int K, int V, int NT>
 int launch_attention4(const PagedAttn& a, const Cache4& c, int most, cudaStream_t st) {
-  constexpr int smem = a4_ring_bytes<K, V, NT>() + sizeof(A4Shared), per_sm = NT == 1 ? 3 : 2;
-  static PerDevice configured;
-  if (once_per_device(configured, [] {
-        const cudaError_t e = cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        return e != cudaSuccess ? e : cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      }) != BX_OK)
-    return BX_ELAUNCH;
   const int n = a.tiles ? a.ntiles : a.M, tallest = a.tiles ? (a.H > 128 ? a.H : 128) : a.H, rows = tallest < most ? tallest : most;
   const int z = ceil_div(rows, 8 * NT);
-  const int cluster = attention4_cluster((i64)n * a.G * z, (i64)a.nblk * a.bs / C4_TOKENS, per_sm);
-  return launch_chained(fl_attention4_kernel<K, V, NT>, dim3((unsigned)n * cluster, a.G, z), 32 * A4_WARPS, smem, st, cluster, a, c, most);
+  const i64 table = (i64)a.nblk * a.bs, seen = a.window > 0 && a.window < table ? a.window + C4_TOKENS : table;
+  const Share4 s = attention4_share((i64)n * a.G * z, (seen + C4_TOKENS - 1) / C4_TOKENS, NT == 2 ? 2 : K + V == 128 ? 4 : 3);
+  const dim3 grid((unsigned)n * s.ctas, a.G, z);
+  return s.warps == 1 ? launch_attention4<K, V, NT, 1>(a, c, most, grid, 1, st) : launch_attention4<K, V, NT, 4>(a, c, most, grid, s.ctas, st);
 }
 
 template <int NT>
