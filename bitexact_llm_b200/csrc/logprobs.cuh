@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_kernel(const LogProbs
   if (ctas > 1) cluster_arrive();
   if (TOP && tid == 0) sh->count = 0, sh->few = 0, sh->threshold = none;
   if (TOP) __syncthreads();
-  launch_next();
   wait_previous();
+  launch_next();
 
   const T* p = static_cast<const T*>(a.logits) + m_row * a.ld;
   LpRow<T> row;

@@ -77,8 +77,8 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
   if (tid == 0) bad_bits = 0;
-  launch_next();
   wait_previous();
+  launch_next();
   const long long most = (long long)a.nblk * a.page;
   const int top = *a.top;
   long long rows = 0;

@@ -6,6 +6,7 @@ import hashlib
 
 import torch
 
+from .logprobs import LogProbs, log_probs
 from .vllm_plugin import sampler
 
 
@@ -17,9 +18,11 @@ def logits_sha(row):
 class Session:
     """B sequences with one block-table row each (page 0 is the null page; a recurrent layer's state of sequence b is slot
     b of its cache). By default every sequence owns a run of pages for max_len tokens. With `pages`, the cache has that
-    many pages for all sequences together: `feed` takes them as a sequence grows and `release` gives them back."""
+    many pages for all sequences together: `feed` takes them as a sequence grows and `release` gives them back. With `on_device`
+    the pool is kept on the device (`pages.DevicePages`): `step` takes pages too, without a host synchronisation, so that it
+    can be captured into a graph; what it finds (no pages left, a sequence beyond max_len) is raised by `check`."""
 
-    def __init__(self, eng, B, max_len, bs=None, perm_seed=None, pages=None):
+    def __init__(self, eng, B, max_len, bs=None, perm_seed=None, pages=None, on_device=False):
         bs = eng.page if bs is None else bs
         self.eng, self.B, self.bs = eng, B, bs
         self.nblk = (max_len + bs - 1) // bs
@@ -30,7 +33,15 @@ class Session:
         if perm_seed is not None:                                  # scattered pages
             g = torch.Generator().manual_seed(perm_seed)
             blocks = blocks[torch.randperm(nb - 1, generator=g)]
-        self.free = None
+        self.free, self.pool = None, None
+        self.rows = torch.arange(B, device=dev)
+        if on_device:
+            if pages is None:
+                raise ValueError("a session on the device has a pool: give its pages")
+            from .pages import DevicePages
+            self.pool = DevicePages(B, self.nblk, pages, bs, dev, blocks)
+            self.bt, self.lens, self.ones = self.pool.bt, self.pool.lens, torch.ones(B, dtype=torch.long, device=dev)
+            return
         if pages is None:
             self.bt = blocks.view(B, self.nblk).to(torch.int32).to(dev)
         else:
@@ -38,7 +49,12 @@ class Session:
             self.free = blocks.tolist()[::-1]
             self.held = [[] for _ in range(B)]
         self.lens = torch.zeros(B, dtype=torch.long, device=dev)
-        self.rows = torch.arange(B, device=dev)
+
+    def check(self):
+        """Raises what the engine or the pool on the device found since the last check (synchronises)."""
+        if self.pool is not None:
+            self.pool.check()
+        self.eng.check()
 
     def _reserve(self, seq, n):
         """Pages for positions 0 .. n - 1 of the sequence."""
@@ -57,6 +73,9 @@ class Session:
     def release(self, seq):
         """The sequence is finished: its pages go back to the pool and its row may serve another one. Nothing is cleared:
         keys beyond a sequence's length carry no weight, and a recurrent state starts from zero at position 0."""
+        if self.pool is not None:
+            self.pool.step(torch.zeros_like(self.lens), 0, self.rows == seq)
+            return
         if self.free is not None:
             self.free += self.held[seq][::-1]
             self.held[seq] = []
@@ -71,8 +90,15 @@ class Session:
         lens = self.lens.tolist()
         todo = [[int(s), torch.as_tensor(t, dtype=torch.long), lens[s]] for s, t in entries]
         assert len({s for s, _, _ in todo}) == len(todo), "a sequence may appear once per call"
-        for s, t, n in todo:
-            self._reserve(s, n + len(t))
+        if self.pool is not None:
+            counts = torch.zeros(self.B, dtype=torch.long)
+            for s, t, _ in todo:
+                counts[s] = len(t)
+            self.pool.step(counts.to(dev), int(counts.sum()))
+            self.pool.check()
+        else:
+            for s, t, n in todo:
+                self._reserve(s, n + len(t))
         out, i = [[] for _ in todo], 0
         while i < len(todo):
             runs, at = [], 0                                       # (entry, sequence, first position, tokens)
@@ -113,7 +139,8 @@ class Session:
             for e, _, _, t in runs:
                 out[e].append(x[row:row + len(t)])
                 row += len(t)
-            self.lens[both[3 * at:3 * at + len(runs)]] = both[3 * at + len(runs):]
+            if self.pool is None:
+                self.lens[both[3 * at:3 * at + len(runs)]] = both[3 * at + len(runs):]
         return [o[0] if len(o) == 1 else torch.cat(o) if o else torch.empty(0, self.eng.D, device=dev) for o in out]
 
     def _slots(self, seq, pos):
@@ -125,6 +152,8 @@ class Session:
         bits, within three limbs) into the paged cache of the given layers (default: all) and sets the sequence's
         length to n: a prefix computed elsewhere, e.g. by another engine or an earlier session."""
         from .vllm_plugin import tri_paged
+        if self.pool is not None:
+            raise ValueError("import_kv: a pool on the device takes its pages by feed, prefill and step")
         dev = self.eng.dev
         k, v = k.to(dev).long().contiguous(), v.to(dev).long().contiguous()
         n = k.shape[0]
@@ -149,6 +178,9 @@ class Session:
         if self.free is not None:
             for b in range(B):
                 self._reserve(b, lens_host[b])
+        if self.pool is not None:                                                  # all pages at once; the lengths advance with them
+            self.pool.step(lens, sum(lens_host))
+            self.pool.check()
         tile_from = 0 if tiles == "always" else self.eng.tiles_from
         step = max(1, chunk_rows // B)
         last = None
@@ -175,13 +207,23 @@ class Session:
             if last is None:
                 last = torch.zeros(B, self.eng.D, dtype=x.dtype, device=dev)
             last[seq[fin]] = x[fin]
-        self.lens += lens
+        if self.pool is None:
+            self.lens += lens
         return last
 
     @torch.no_grad()
-    def step(self, tokens, pos=None):
+    def step(self, tokens, pos=None, active=None):
         """One decode step: tokens int64 [B] at positions `pos` (default: the lengths tracked on the device).
-        Returns the residual rows [B, D]. (With a page pool the pages must be there: `feed` takes them as needed.)"""
+        Returns the residual rows [B, D]. (With a page pool on the host the pages must be there: `feed` takes them as needed; a
+        pool on the device takes them here. There `active` bool [B] tells which sequences take part; the others' rows are not theirs.)"""
+        if self.pool is not None:
+            if pos is not None:
+                raise ValueError("step: a pool on the device keeps the positions")
+            t = self.pool.step(self.ones if active is None else active.long(), self.B)
+            x = self.eng.forward(self.kvs, tokens[t.seq], t.pos, t.slot, self.bt, t.seq)
+            return x[t.last.clamp(min=0)]
+        if active is not None:
+            raise ValueError("step: active sequences need a pool on the device")
         pos = self.lens.clone() if pos is None else pos
         x = self.eng.forward(self.kvs, tokens, pos, self._slots(self.rows, pos), self.bt, self.rows)
         self.lens += 1
@@ -250,9 +292,10 @@ class GraphHostStep:
 
 
 @torch.no_grad()
-def generate(eng, prompts, max_new, tn=0, td=1, seeds=None, hashes=True, max_len=None, perm_seed=None, lens=None):
+def generate(eng, prompts, max_new, tn=0, td=1, seeds=None, hashes=True, max_len=None, perm_seed=None, lens=None, logprobs=None):
     """prompts int64 [B, P] (right-padded, true lengths `lens`); generated token t of sequence b uses the noise
-    keyed (seeds[b], t). Returns (tokens [B, max_new] on the host, list of per-position hash lists or None)."""
+    keyed (seeds[b], t). Returns (tokens [B, max_new] on the host, list of per-position hash lists or None); with logprobs = k also
+    the `logprobs.LogProbs` of the tokens with their k best alternatives, [B, max_new] and [B, max_new, k] on the host."""
     B, P = prompts.shape
     dev = eng.dev
     seeds = list(range(B)) if seeds is None else seeds
@@ -261,16 +304,39 @@ def generate(eng, prompts, max_new, tn=0, td=1, seeds=None, hashes=True, max_len
     rows = torch.zeros(B, 4, dtype=torch.long, device=dev)
     rows[:, 0] = torch.tensor(seeds, device=dev)
     rows[:, 2], rows[:, 3] = tn, td
-    toks, shas = [], [[] for _ in range(B)]
+    toks, shas, probs = [], [[] for _ in range(B)], []
     for t in range(max_new):
         lg = eng.logits(h)
         rows[:, 1] = t
         y = sampler.sample_rows(lg, rows, eng.ln, eng.FR)
         toks.append(y)
+        if logprobs is not None:
+            probs.append(log_probs(lg, y, logprobs, eng.FR))
         if hashes:
             for b in range(B):
                 shas[b].append(logits_sha(lg[b]))
         if t + 1 < max_new:
             h = ses.step(y)
     eng.check()
-    return torch.stack(toks, 1).cpu(), (shas if hashes else None)
+    out = torch.stack(toks, 1).cpu(), (shas if hashes else None)
+    return out if logprobs is None else (*out, LogProbs(*(torch.stack(p, 1).cpu() for p in zip(*probs))))
+
+
+@torch.no_grad()
+def score(eng, prompts, top=0, chunk_rows=1024, max_len=None):
+    """prompts: lists of token ids -> one `logprobs.LogProbs` per prompt on the host: of every token but the first, given those before it
+    (entry i is token i + 1), with the `top` best alternatives at its place."""
+    prompts = [torch.as_tensor(p, dtype=torch.long) for p in prompts]
+    if any(len(p) < 1 for p in prompts):
+        raise ValueError("score: a prompt has at least one token")
+    ses = Session(eng, len(prompts), max_len or max(map(len, prompts)))
+    out = []
+    for p, x in zip(prompts, ses.feed(list(enumerate(prompts)))):
+        want = p[1:].to(eng.dev)
+        parts = [log_probs(torch.empty(0, eng.V, dtype=torch.long, device=eng.dev), want[:0], top, eng.FR)]      # the shapes of a prompt of one token
+        for i in range(0, len(want), chunk_rows):
+            n = want[i:i + chunk_rows]
+            parts.append(log_probs(eng.logits(x[i:i + len(n)]), n, top, eng.FR))
+        out.append(LogProbs(*(torch.cat(v).cpu() for v in zip(*parts))))
+    eng.check()
+    return out

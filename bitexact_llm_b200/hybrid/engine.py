@@ -24,10 +24,11 @@ class HybridEngine(TokenRowEngine):
     page = 64               # the attention kernel's key block: one copy per page and column block
     tiles_from = 0
 
-    def __init__(self, spec, weights, dev="cuda", dtype="bfloat16", n_layers=None):
+    def __init__(self, spec, weights, dev="cuda", dtype="bfloat16", n_layers=None, cache=None):
         """spec: ModelSpec; weights: {'embed', 'head', 'final', 'layers': [{'norm1', 'norm2', 'mixer', 'ff': dicts of the
         mechanism, 'hc1', 'hc2'}]} as tensors (a design's `read_weights`). Norms are (w, b), with streams w around zero;
-        'hc<q>' are the dicts 'in', 'out', 'mix' of a sublayer's streams. n_layers: only the first runs."""
+        'hc<q>' are the dicts 'in', 'out', 'mix' of a sublayer's streams. n_layers: only the first runs. cache: None (keys and values
+        in the model's format) or 'fp4' (grouped-query layers keep them in 4 bits, in pages of multiples of 64 tokens)."""
         self.dev, self.spec = torch.device(dev), spec
         self.dtype, _ = ops.DTYPES[dtype]
         self.D, self.V = spec.width, spec.vocab
@@ -45,6 +46,14 @@ class HybridEngine(TokenRowEngine):
             made[i] = (sub(w, 1), make(MIXERS, s.mixer, w["mixer"]), sub(w, 2) if s.ff is not None else None,
                        make(FEED_FORWARDS, s.ff, w["ff"]))
         self.layers = [made[i] for i in runs]
+        if cache not in (None, "fp4"):
+            raise ValueError(f"cache {cache!r}: None or 'fp4'")
+        if cache == "fp4":
+            layers = [mixer for _, mixer, _, _ in self.layers if isinstance(mixer, Attention)]
+            if not layers:
+                raise ValueError("cache 'fp4': the model has no grouped-query attention")
+            for mixer in layers:
+                mixer.cache4 = True
         counters = max([ff.counters for _, _, _, ff in self.layers if ff is not None], default=0)
         self.counts = torch.zeros(max(1, counters), dtype=torch.int32, device=self.dev)
         self._ln = None

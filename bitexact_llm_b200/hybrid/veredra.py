@@ -65,6 +65,6 @@ def read_weights(spec, t):
     return {"embed": t["embed"], "head": t["head"], "final": t["final.norm"], "layers": layers}
 
 
-def load(cfg, tensors, dev="cuda", dtype="bfloat16", n_layers=None):
+def load(cfg, tensors, dev="cuda", dtype="bfloat16", n_layers=None, cache=None):
     spec = read_config(cfg)
-    return HybridEngine(spec, read_weights(spec, tensors), dev, dtype, n_layers)
+    return HybridEngine(spec, read_weights(spec, tensors), dev, dtype, n_layers, cache)

@@ -2,7 +2,7 @@
 `engine_base`, so the decode loop, the command line and the trace runner treat all of them alike.
 
   Fedatar            hybrid.fedatar   dtype bfloat16 (default) or float32
-  Veredra            hybrid.veredra   dtype bfloat16 (default) or float32
+  Veredra            hybrid.veredra   dtype bfloat16 (default) or float32; cache fp4
   LlamaForCausalLM   integer engines  dtype exact (default: original bf16 weights as limbs) or int8
 
 A folder holds config.json and model.safetensors; the integer engines also take constants.bx (`constfile`), which
@@ -32,6 +32,7 @@ def _tensors(folder):
 class FedatarFamily:
     dtypes, libraries = ("bfloat16", "float32"), ("float",)
     serving_dtype = "bfloat16"
+    caches = ()                 # formats of keys and values beside the model's own
 
     @staticmethod
     def load(folder, cfg, dev, dtype, max_len):
@@ -40,15 +41,18 @@ class FedatarFamily:
 
 
 class VeredraFamily(FedatarFamily):
+    caches = ("fp4",)
+
     @staticmethod
-    def load(folder, cfg, dev, dtype, max_len):
+    def load(folder, cfg, dev, dtype, max_len, cache=None):
         from .hybrid import veredra
-        return veredra.load(cfg, _tensors(folder), dev, dtype)
+        return veredra.load(cfg, _tensors(folder), dev, dtype, cache=cache)
 
 
 class LlamaFamily:
     dtypes, libraries = ("exact", "int8"), ("integer",)
     serving_dtype = "exact"
+    caches = ()
 
     @staticmethod
     def load(folder, cfg, dev, dtype, max_len):
@@ -87,11 +91,16 @@ def family(cfg):
     raise ValueError(f"unknown architecture {names}; known: {sorted(FAMILIES)}")
 
 
-def load(folder, dev="cuda", dtype=None, max_len=2048):
-    """-> engine. dtype None: the family's serving format; max_len sizes position tables where a family has them."""
+def load(folder, dev="cuda", dtype=None, max_len=2048, cache=None):
+    """-> engine. dtype None: the family's serving format; max_len sizes position tables where a family has them; cache: 'fp4' keeps
+    keys and values in 4 bits where a family can, None in the model's own format."""
     cfg = read_config(folder)
     fam = family(cfg)
     dtype = fam.serving_dtype if dtype is None else dtype
     if dtype not in fam.dtypes:
         raise UnsupportedDtype(f"{dtype}: this model runs in {', '.join(fam.dtypes)}")
-    return fam.load(folder, cfg, dev, dtype, max_len)
+    if cache is None:
+        return fam.load(folder, cfg, dev, dtype, max_len)
+    if cache not in fam.caches:
+        raise UnsupportedDtype(f"cache {cache}: this model has none in that format")
+    return fam.load(folder, cfg, dev, dtype, max_len, cache)

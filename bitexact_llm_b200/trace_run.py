@@ -1,6 +1,6 @@
 """Replays a trace of token ids through a model and writes logits:
 
-    bin/trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N
+    bin/trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--cache fp4]
 
 Standard input holds one step per line, {"step": 0, "entries": [{"id": "a", "tokens": [5, 17], "want": [0, 1]}],
 "end": ["a"]}: the next tokens of each request, the places among them whose logits are written to DIR/<step>.f32 (float32,
@@ -23,6 +23,7 @@ def parse(argv=None):
     ap.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
     ap.add_argument("--out", required=True)
     ap.add_argument("--max-tokens", type=int, default=4096, help="tokens that live requests hold at any time")
+    ap.add_argument("--cache", default=None, help="format of keys and values: fp4 (default: the model's own)")
     return ap.parse_args(argv)
 
 
@@ -64,7 +65,7 @@ def main(argv=None):
         build.build(target=target)
     from .decode import Session
     n = max(1, args.max_tokens)
-    eng = registry.load(args.model, dtype=dtype, max_len=n)
+    eng = registry.load(args.model, dtype=dtype, max_len=n, cache=args.cache)
     replay = Replay(Session(eng, SLOTS, n, pages=(n + eng.page - 1) // eng.page + SLOTS))
     for line in sys.stdin:
         if not line.strip():
