@@ -450,10 +450,10 @@ int exact_linear_auto(int M, int N, int K, bool residual) {
 
 // CTAs that share a row: the power of two with the least estimated time, rounds of the resident CTAs (four to an SM) times a CTA's
 // part of the row at its share of the memory's rate and what a CTA costs beside it (us, measured as the slope over many small
-// parts: joining 4, with the best list 9).
+// parts: joining 5, with the best list 9).
 int log_probs_cluster(int M, int V, int bytes, bool top) {
   const long long resident = 4ll * device_sms();
-  const double row = (double)V * bytes / (6.0e6 / resident), own = top ? 9.0 : 4.0;
+  const double row = (double)V * bytes / (6.0e6 / resident), own = top ? 9.0 : 5.0;
   int best = 1;
   double least = 0.0;
   for (int c = 1; c <= LP_MAX_CLUSTER; c *= 2) {
@@ -1856,7 +1856,8 @@ int bx_step_tables(const int64_t* lens, const int64_t* counts, const uint8_t* dr
     return BX_EARG;
   static PerDevice configured;
   if (once_per_device(configured, [] {
-        return cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * ST_MAX_REQUESTS);
+        const cudaError_t e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * ST_MAX_REQUESTS);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       }) != BX_OK)
     return BX_ELAUNCH;
   // a CTA for every two rows of a thread

@@ -121,25 +121,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Four bytes of two e2m1 codes each -> four pairs of fp16.
-__device__ __forceinline__ void e2m1_pairs(uint32_t w, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 x, y, z, w;\n\t"
-      "mov.b32 {x, y, z, w}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, x;\n\tcvt.rn.f16x2.e2m1x2 %1, y;\n\tcvt.rn.f16x2.e2m1x2 %2, z;\n\tcvt.rn.f16x2.e2m1x2 %3, w;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(w));
-}
-// The two e4m3 scales in the low half of w -> a pair of fp16.
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);

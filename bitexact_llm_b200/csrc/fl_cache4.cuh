@@ -34,8 +34,11 @@ struct Cache4 {
   int nb, G, page, dim, vdim, K, V;
 
   __host__ __device__ int bytes() const { return 36 * (K + V) + 2 * C4_TOKENS; }
+  __device__ __forceinline__ bool has(i64 slot) const { return slot >= 0 && slot < (i64)nb * page; }
   __device__ __forceinline__ uint8_t* block(i64 slot, int g) const {
-    return p + ((slot / page * G + g) * (page / C4_TOKENS) + slot % page / C4_TOKENS) * bytes();
+    // the division in 32 bits where the slots of the cache have no more (a 64-bit one is some hundred instructions)
+    const i64 n = (i64)nb * page <= 0x7fffffffll ? (i64)((uint32_t)slot / (uint32_t)page) : slot / page;
+    return p + ((n * G + g) * (page / C4_TOKENS) + (int)(slot - n * page) / C4_TOKENS) * bytes();
   }
   __device__ __forceinline__ int key_scale(int tok, int j) const {
     return 32 * K + ((tok / 16 * 2 + tok % 2) * (K / 16) + j) * 8 + tok % 16 / 2;
@@ -45,6 +48,27 @@ struct Cache4 {
   __device__ __forceinline__ int key_exp(int tok) const { return 36 * (K + V) + tok; }
   __device__ __forceinline__ int value_exp(int tok) const { return 36 * (K + V) + C4_TOKENS + tok; }
 };
+
+// Four bytes of two e2m1 codes each -> four pairs of fp16. (The compiler of CUDA 12.9 gives zeros for a word that it knows to be a zero-extended
+// 16-bit load: such a one is handed over twice, in both halves.)
+__device__ __forceinline__ void e2m1_pairs(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 x, y, z, w;\n\t"
+      "mov.b32 {x, y, z, w}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, x;\n\tcvt.rn.f16x2.e2m1x2 %1, y;\n\tcvt.rn.f16x2.e2m1x2 %2, z;\n\tcvt.rn.f16x2.e2m1x2 %3, w;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+// The two e4m3 scales in the low half of w -> a pair of fp16.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 __device__ __forceinline__ float c4_power(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -58,15 +82,17 @@ __device__ __forceinline__ float c4_code(int c) {
   return c & 8 ? -v : v;
 }
 
-// The smallest scale of which 6 steps reach `most` (below 2048): an estimate from below, and at most two steps up.
+// The smallest scale of which 6 steps reach `most` (below 2048): an estimate from below, which is one less unless it is exact (two where a
+// 32-bit `most` is the next number above a multiple).
+template <class T>
 __device__ __forceinline__ int c4_scale_for(float most) {
   const float f = __fmul_rd(most, 0.16666666f);
   int c = f < 0.015625f ? (int)(f * 512.0f) : (__float_as_int(f) - (120 << 23)) >> 20;
   c += 6.0f * c4_scale(c) < most;
-  c += 6.0f * c4_scale(c) < most;
+  if constexpr (sizeof(T) == 4) c += 6.0f * c4_scale(c) < most;
   return c;
 }
-// Codes of four entries in steps of `step` (inv = 1 / step rounded; both 0 where the block is): the quotient, corrected by its exact
+// Codes of four entries in steps of `step` (inv = about 1 / step; both 0 where the block is): the quotient, corrected by its exact
 // remainder, is the correctly rounded one, and exact where it is a tie. The entries of bf16 rows come no nearer to a tie without being
 // one than 2^-12 of it; those of 32-bit rows may round to one, and are set beside it by the sign of what remains.
 template <class T>
@@ -115,15 +141,23 @@ struct C4Row {
       }
     }
   }
-  // -> the largest finite magnitude of the row; whether all of the lane's entries are finite. Those that are not become 0.
-  __device__ __forceinline__ float most(bool& fine) {
+  // -> the largest magnitude of the row as bits, which order like the numbers; NaN and infinities are above all of them.
+  __device__ __forceinline__ uint32_t most() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = max(m, __float_as_uint(x[i][k]) & 0x7fffffffu);
+    return __reduce_max_sync(0xffffffffu, m);
+  }
+  // Entries that are no numbers become 0, those beyond 2^127 that; -> the largest magnitude of the row then.
+  __device__ __noinline__ float mend() {
     float m = 0.0f;
-    fine = true;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (!(fabsf(x[i][k]) < INFINITY)) fine = false, x[i][k] = 0.0f;
+        if (!(fabsf(x[i][k]) < INFINITY)) x[i][k] = 0.0f;
         x[i][k] = fminf(fmaxf(x[i][k], -1.7014118e38f), 1.7014118e38f);
         m = fmaxf(m, fabsf(x[i][k]));
       }
@@ -135,9 +169,9 @@ struct C4Row {
     float m = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    scale = c4_scale_for(m);
+    scale = c4_scale_for<T>(m);
     const float step = c4_scale(scale);
-    return c4_codes<T>(y, step, step > 0.0f ? __frcp_rn(step) : 0.0f);
+    return c4_codes<T>(y, step, step > 0.0f ? __fdividef(1.0f, step) : 0.0f);
   }
 };
 
@@ -164,14 +198,15 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
   constexpr int PITCH = ROWS + 4;      // bytes of a value column of the CTA's rows
   extern __shared__ __align__(16) uint8_t s4_smem[];
   __shared__ i64 slots[ROWS];
+  __shared__ uint8_t* blocks[ROWS];                        // of the rows' tokens; NULL: a row that is left out
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y, row0 = blockIdx.x * ROWS;
   const Cache4& c = a.c;
-  const i64 most_slots = (i64)c.nb * c.page;
   launch_next();
   wait_previous();
   if (threadIdx.x < ROWS) {
     const i64 s = row0 + (int)threadIdx.x < a.M ? a.slot[row0 + threadIdx.x] : -1;
-    slots[threadIdx.x] = s >= 0 && s < most_slots ? s : -1;
+    slots[threadIdx.x] = c.has(s) ? s : -1;
+    blocks[threadIdx.x] = c.has(s) ? c.block(s, g) : nullptr;
   }
   __syncthreads();
   const int columns = c.V / 2 + c.V / 16 + 1;              // of value bytes: codes, scales, the exponent
@@ -188,10 +223,11 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
     fetch(r + S4_THREADS / 32);
     if (slots[r] < 0) continue;
     const int tok = (int)(slots[r] % C4_TOKENS);
-    uint8_t* block = c.block(slots[r], g);
-    bool fine_k, fine_v;
-    const float most_k = k.most(fine_k), most_v = v.most(fine_v);
-    const bool bad = !__all_sync(0xffffffffu, fine_k && fine_v);
+    uint8_t* block = blocks[r];
+    const uint32_t bits_k = k.most(), bits_v = v.most();
+    const bool bad = max(bits_k, bits_v) >= 0x7f800000u;
+    float most_k = __uint_as_float(bits_k), most_v = __uint_as_float(bits_v);
+    if (max(bits_k, bits_v) > 0x7f000000u) most_k = k.mend(), most_v = v.mend();
     const int ek = c4_exponent(most_k), ev = c4_exponent(most_v);
     const float uk = c4_power(-ek), uv = bad ? 0.0f : c4_power(-ev);
 #pragma unroll
@@ -238,23 +274,24 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
     const int col = i % columns, r0 = i / columns * 16;
     const uint8_t* from = s4_smem + col * PITCH + r0;
     const i64 s0 = slots[r0];
-    auto at = [&](i64 s) { return c.block(s, g) + (col < columns - 1 ? 36 * c.K + col * C4_TOKENS : 36 * (c.K + c.V) + C4_TOKENS) + s % C4_TOKENS; };
+    const int place = col < columns - 1 ? 36 * c.K + col * C4_TOKENS : 36 * (c.K + c.V) + C4_TOKENS;
+    auto at = [&](int r) { return blocks[r] + place + (int)(slots[r] % C4_TOKENS); };
     bool run = s0 >= 0 && s0 % 16 == 0;
 #pragma unroll
     for (int k = 1; k < 16; ++k) run &= slots[r0 + k] == s0 + k;
     const uint32_t* w = reinterpret_cast<const uint32_t*>(from);
     if (run) {
-      *reinterpret_cast<uint4*>(at(s0)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(at(r0)) = make_uint4(w[0], w[1], w[2], w[3]);
       continue;
     }
     for (int k = 0; k < 16; k += 4) {
       const i64 s = slots[r0 + k];
       if (s >= 0 && s % 4 == 0 && slots[r0 + k + 1] == s + 1 && slots[r0 + k + 2] == s + 2 && slots[r0 + k + 3] == s + 3) {
-        *reinterpret_cast<uint32_t*>(at(s)) = w[k / 4];
+        *reinterpret_cast<uint32_t*>(at(r0 + k)) = w[k / 4];
         continue;
       }
       for (int n = k; n < k + 4; ++n)
-        if (slots[r0 + n] >= 0) *at(slots[r0 + n]) = from[n];
+        if (slots[r0 + n] >= 0) *at(r0 + n) = from[n];
     }
   }
 }
@@ -277,28 +314,36 @@ template <class T>
 __global__ void __launch_bounds__(32 * R4_WARPS) fl_read4_kernel(const Cache4 c, const i64* slot, T* k, T* v, i64 rows) {
   launch_next();
   wait_previous();
-  const i64 at = (i64)blockIdx.x * R4_WARPS + (threadIdx.x >> 5);
+  const uint32_t at = blockIdx.x * R4_WARPS + (threadIdx.x >> 5);          // below 2^31 + 8
   const int lane = threadIdx.x & 31;
   if (at >= rows) return;
-  const i64 s = slot[at / c.G];
-  const bool in = s >= 0 && s < (i64)c.nb * c.page;
+  const uint32_t m = at / (uint32_t)c.G;
+  const i64 s = slot[m];
+  const bool in = c.has(s);
   const int tok = in ? (int)(s % C4_TOKENS) : 0;
-  const uint8_t* b = c.block(in ? s : 0, (int)(at % c.G));
+  const uint8_t* b = c.block(in ? s : 0, (int)(at - m * c.G));
   const float pk = in ? __int_as_float(b[c.key_exp(tok)] << 23) : 0.0f, pv = in ? __int_as_float(b[c.value_exp(tok)] << 23) : 0.0f;
-  for (int d = 4 * lane; d < c.dim; d += 128) {
-    const int w = *reinterpret_cast<const uint16_t*>(b + tok * (c.K / 2) + d / 2);
-    const float f = c4_scale(b[c.key_scale(tok, d / 16)] & 127);
+  auto put = [&](T* to, int d, int n, uint32_t codes, uint32_t scale, float power) {
+    uint32_t h[4];
+    e2m1_pairs(codes, h);
+    const uint32_t f = e4m3_pair((scale & 127) * 0x0101u);
     float x[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = in ? c4_code(w >> (4 * q) & 15) * f * pk : 0.0f;
-    c4_put(k + at * c.dim, d, c.dim, x);
-  }
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t v = hmul2(h[q], f);
+      const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&v));
+      x[2 * q] = in ? w.x * power : 0.0f, x[2 * q + 1] = in ? w.y * power : 0.0f;
+    }
+    c4_put(to, d, n, x);
+  };
+  for (int d = 4 * lane; d < c.dim; d += 128)
+    put(k + (i64)at * c.dim, d, c.dim, *reinterpret_cast<const uint16_t*>(b + tok * (c.K / 2) + d / 2) * 0x10001u, b[c.key_scale(tok, d / 16)], pk);
   for (int d = 4 * lane; d < c.vdim; d += 128) {
-    const float f = c4_scale(b[c.value_scale(tok, d / 16)] & 127);
-    float x[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = in ? c4_code(b[c.value_code(tok, d / 16, d % 8 + q)] >> (d % 16 / 8 * 4) & 15) * f * pv : 0.0f;
-    c4_put(v + at * c.vdim, d, c.vdim, x);
+    const uint8_t* from = b + c.value_code(tok, d / 16, d % 8);
+    const int half = d % 16 / 8 * 4;
+    const uint32_t codes = (from[0] >> half & 15) | (from[C4_TOKENS] >> half & 15) << 4 | (from[2 * C4_TOKENS] >> half & 15) << 8 |
+                           (from[3 * C4_TOKENS] >> half & 15) << 12;
+    put(v + (i64)at * c.vdim, d, c.vdim, codes, b[c.value_scale(tok, d / 16)], pv);
   }
 }
 

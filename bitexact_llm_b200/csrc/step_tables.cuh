@@ -15,7 +15,7 @@
 
 namespace bx {
 
-constexpr int ST_THREADS = 1024, ST_MAX_REQUESTS = 8192, ST_MAX_CLUSTER = 8;
+constexpr int ST_THREADS = 1024, ST_MAX_REQUESTS = 8192, ST_MAX_CLUSTER = 16;
 
 struct StepTables {
   const long long *lens, *counts;
@@ -51,17 +51,39 @@ __device__ __forceinline__ void st_scan(long long& r, int& p, int& t, int lane) 
   }
 }
 
-// Row i, of request b (-1: padding). `full`: pages on the stack before any were taken.
-__device__ __forceinline__ void st_row(const StepTables& a, int i, int b, const int* row_end, const int* take_end, const int* base, int full) {
-  if (b < 0) {
-    a.seq[i] = 0, a.pos[i] = 0, a.slot[i] = -1;
+// N rows from i on, of which those below `live` are tokens: what has to be looked up first, then the stores (a load is not moved in front
+// of a store that might be to the same place). `full`: pages on the stack before any were taken.
+template <int N>
+__device__ __forceinline__ void st_rows(const StepTables& a, int i, int live, const int* row_end, const int* take_end, const int* base, int full) {
+  int b = i < live ? st_owner(row_end, a.B, i) : 0, owner[N], pos[N], page[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    owner[k] = pos[k] = 0, page[k] = -1;
+    if (i + k >= live) continue;
+    while (row_end[b] <= i + k) ++b;
+    const int start = base[b], held = st_pages(start, a.page);
+    owner[k] = b;
+    pos[k] = start + i + k - (b ? row_end[b - 1] : 0);
+    const int block = (int)((unsigned)pos[k] / (unsigned)a.page);
+    page[k] = block < held ? a.bt[b * a.bt_stride + block]
+                           : *const_cast<volatile int*>(a.free + full - 1 - (b ? take_end[b - 1] : 0) - (block - held));
+  }
+  long long slot[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    slot[k] = i + k < live ? (long long)page[k] * a.page + pos[k] - (int)((unsigned)pos[k] / (unsigned)a.page) * a.page : -1;
+  if (N % 2 == 0 && i + N <= a.rows && ((reinterpret_cast<uintptr_t>(a.seq) | reinterpret_cast<uintptr_t>(a.pos) | reinterpret_cast<uintptr_t>(a.slot)) & 15) == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      *reinterpret_cast<longlong2*>(a.seq + i + k) = make_longlong2(owner[k], owner[k + 1 < N ? k + 1 : k]);
+      *reinterpret_cast<longlong2*>(a.pos + i + k) = make_longlong2(pos[k], pos[k + 1 < N ? k + 1 : k]);
+      *reinterpret_cast<longlong2*>(a.slot + i + k) = make_longlong2(slot[k], slot[k + 1 < N ? k + 1 : k]);
+    }
     return;
   }
-  const int start = base[b], pos = start + i - (b ? row_end[b - 1] : 0);
-  const int held = st_pages(start, a.page), block = (int)((unsigned)pos / (unsigned)a.page);
-  const int page = block < held ? a.bt[b * a.bt_stride + block]
-                                : *const_cast<volatile int*>(a.free + full - 1 - (b ? take_end[b - 1] : 0) - (block - held));
-  a.seq[i] = b, a.pos[i] = pos, a.slot[i] = (long long)page * a.page + (pos - block * a.page);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (i + k < a.rows) a.seq[i + k] = owner[k], a.pos[i + k] = pos[k], a.slot[i + k] = slot[k];
 }
 
 __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTables a) {
@@ -165,23 +187,12 @@ __global__ void __launch_bounds__(ST_THREADS) step_tables_kernel(const StepTable
       const int nth = i - (b ? take_end[b - 1] : 0);
       a.bt[b * a.bt_stride + st_pages(base[b], a.page) + nth] = stack[full - 1 - i];
     }
-  // PER rows in a run for each thread: one bisection, and mostly one page
-  constexpr int PER = 4;
-  const int runs = (a.rows + PER - 1) / PER, live = bad ? 0 : (int)rows;
+  // few rows: one a thread; else runs of four, one bisection and mostly one page each
+  const int live = bad ? 0 : (int)rows;
   if (a.rows <= 2 * step) {
-    for (int i = at; i < a.rows; i += step) st_row(a, i, i < live ? st_owner(row_end, a.B, i) : -1, row_end, take_end, base, full);
-    return;
-  }
-  for (int run = at; run < runs; run += step) {
-    int i = run * PER, b = i < live ? st_owner(row_end, a.B, i) : -1;
-#pragma unroll
-    for (int k = 0; k < PER; ++k, ++i) {
-      if (i >= a.rows) break;
-      if (i >= live) b = -1;
-      else
-        while (row_end[b] <= i) ++b;
-      st_row(a, i, b, row_end, take_end, base, full);
-    }
+    for (int i = at; i < a.rows; i += step) st_rows<1>(a, i, live, row_end, take_end, base, full);
+  } else {
+    for (int i = 4 * at; i < a.rows; i += 4 * step) st_rows<4>(a, i, live, row_end, take_end, base, full);
   }
 }
 
