@@ -15,13 +15,15 @@
 // grows by more than 2^8 since the last time. Few tiles (decoding): the keys of a tile are split over blockIdx.y, and a
 // second kernel joins the parts.
 //
-// A 4-bit cache (FOUR; fl_cache4.cuh) has two more warps, which make fp16 operands of a block in shared memory from its codes: a raw
-// block arrives by one bulk copy while the warps wait for a free stage, keys become K-major rows as a TMA copy would leave them,
-// values, whose codes lie along the tokens, a K-major V^T. An entry is its code times its scale times 2^(e - E), with E the largest
-// exponent of the block's keys (it goes into the scores), or of the values so far (the accumulator is rescaled when it grows): exact
-// for rows within 2^14 of the largest one, off by 2^-36 of that one's largest entry beyond. The queries are turned to fp16 in place,
-// each row times a power of two, and weights are held times 2^6. It is for tiles of many query rows, which share that work; short
-// tiles have the kernel of fl_attention4.cuh, and each of the two leaves the other's tiles alone.
+// A 4-bit cache (FOUR; fl_cache4.cuh): the softmax warps also make the fp16 operands of the next block in shared memory from its codes,
+// in front of a block's softmax, so that its scores are computed meanwhile. A raw block arrives by one bulk copy; keys become
+// K-major rows as a TMA copy would leave them, values, whose codes lie along the tokens, a K-major V^T. An entry is its code times its
+// scale times 2^(e - E), with E the largest exponent of the block's keys (it goes into the scores), or of the values so far (the
+// accumulator is rescaled when it grows): exact for rows within 2^14 of the largest one, off by 2^-36 of that one's largest entry
+// beyond. The queries are turned to fp16 in place, each row times a power of two, and weights are held times 2^6. It is for tiles of
+// many query rows, which share that work; short tiles have the kernel of fl_attention4.cuh, and each of the two leaves the
+// other's tiles alone. (Two or four warps of their own for the operands were slower: they were a chain of latencies of 4200 cycles a
+// block, where eight warps with other work beside it take turns.)
 #pragma once
 
 #include "fl_attention4.cuh"
@@ -51,11 +53,7 @@ struct LatentShared {
   uint64_t full[LT_MAX_STAGES], empty[LT_MAX_STAGES], raw_full;
   uint64_t s_full[2], p_full[2], pv_done[2];
   float row_max[2][SHARE][128], row_den[SHARE][128];
-  // FOUR: the queries are fp16; the largest key exponent of a stage's block, the largest value exponent so far; of the query rows
-  uint64_t q_ready;
-  int exps[LT_MAX_STAGES][2];
-  short q_exp[128];
-  alignas(16) uint32_t scales[LT_VCOLS / 32 * LT_KEYS / 2];
+  uint64_t q_ready, raw_empty;                           // FOUR: the queries are fp16; the raw block is used
   uint32_t tmem_base, abort_flag;
 };
 
@@ -70,10 +68,7 @@ template <int PARTS>
 __device__ __forceinline__ void quarter_barrier(int quarter) {
   asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * PARTS) : "memory");
 }
-constexpr int LT_LOADERS = 2;                            // warps that make operands from codes
-__host__ __device__ constexpr int lt_threads(int parts, bool four = false) { return 64 + 128 * parts + (four ? 32 * LT_LOADERS : 0); }
-
-__device__ __forceinline__ void loaders_barrier() { asm volatile("bar.sync 9, %0;" ::"n"(32 * LT_LOADERS) : "memory"); }
+__host__ __device__ constexpr int lt_threads(int parts) { return 64 + 128 * parts; }
 
 // A pair of fp16 scales times 2^-u, u in the halves of a word; deep: some u is beyond 14, where 2^-u is no normal fp16 any more.
 __device__ __forceinline__ uint32_t scaled_down(uint32_t scale, uint32_t u, bool deep) {
@@ -83,54 +78,42 @@ __device__ __forceinline__ uint32_t scaled_down(uint32_t scale, uint32_t u, bool
   return scale;
 }
 
-// One block's keys, by all loader threads: thread (row, column box) writes 64 entries of a row, 16 bytes at a time where a
-// 128-byte-swizzled copy would put them. deep: some row is more than 2^14 below E. What is read comes first: a load is not
-// moved in front of a store that might be to the same place.
+// One block's keys, by T threads: thread (row, 32 entries) writes four chunks of 16 bytes where a 128-byte-swizzled copy would put
+// them. deep: some row is more than 2^14 below E. What is read comes first: a load is not moved in front of a store that might
+// be to the same place.
+template <int T>
 __device__ __forceinline__ void operand_keys(const uint8_t* __restrict__ raw, uint8_t* __restrict__ st, const Cache4& c, int E, bool deep, int tid) {
   const int r = tid % LT_KEYS;
   const uint32_t down = (E - min((int)raw[c.key_exp(r)], E)) * 0x00010001u;
-  for (int box = tid / LT_KEYS; box < c.K / 64; box += 32 * LT_LOADERS / LT_KEYS) {
-    const uint4* codes = reinterpret_cast<const uint4*>(raw + r * (c.K / 2) + box * 32);
-    const uint4 v0 = codes[0], v1 = codes[1];
-    const uint32_t w[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-    uint32_t scale[4];
+  for (int part = tid / LT_KEYS; part < c.K / 32; part += T / LT_KEYS) {
+    const uint4 v = *reinterpret_cast<const uint4*>(raw + r * (c.K / 2) + part * 16);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t scale[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) scale[j] = (raw[c.key_scale(r, box * 4 + j)] & 127) * 0x0101u;
+    for (int j = 0; j < 2; ++j) scale[j] = (raw[c.key_scale(r, part * 2 + j)] & 127) * 0x0101u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) scale[j] = scaled_down(e4m3_pair(scale[j]), down, deep);
-    uint8_t* row = st + box * (LT_KEYS * 128) + r * 128;
+    for (int j = 0; j < 2; ++j) scale[j] = scaled_down(e4m3_pair(scale[j]), down, deep);
+    uint8_t* row = st + part / 2 * (LT_KEYS * 128) + r * 128;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < 4; ++k) {
       uint32_t h[4];
       e2m1_pairs(w[k], h);
-      *reinterpret_cast<uint4*>(row + ((k ^ (r & 7)) << 4)) =
+      *reinterpret_cast<uint4*>(row + (((part % 2 * 4 + k) ^ (r & 7)) << 4)) =
           make_uint4(hmul2(h[0], scale[k / 2]), hmul2(h[1], scale[k / 2]), hmul2(h[2], scale[k / 2]), hmul2(h[3], scale[k / 2]));
     }
   }
 }
-// Scales of its values as fp16 pairs of tokens relative to E: word (j, pair) for entries 16 j .. 16 j + 15.
-__device__ __forceinline__ void operand_scales(const uint8_t* __restrict__ raw, uint32_t* __restrict__ scales, const Cache4& c, int E, bool deep,
-                                               int tid) {
-  const uint32_t most = (uint32_t)E * 0x00010001u;
-  for (int u = tid; u < c.V / 16 * (LT_KEYS / 4); u += 32 * LT_LOADERS) {                 // four tokens
-    const int j = u / (LT_KEYS / 4), t = u % (LT_KEYS / 4) * 4;
-    const uint32_t s = *reinterpret_cast<const uint32_t*>(raw + 36 * c.K + 32 * c.V + j * C4_TOKENS + t);
-    const uint32_t e = *reinterpret_cast<const uint32_t*>(raw + 36 * (c.K + c.V) + C4_TOKENS + t);
-    const uint32_t lo = scaled_down(e4m3_pair(s), most - __vminu2(__byte_perm(e, 0, 0x4140), most), deep);
-    const uint32_t hi = scaled_down(e4m3_pair(s >> 16), most - __vminu2(__byte_perm(e, 0, 0x4342), most), deep);
-    *reinterpret_cast<uint2*>(scales + j * (LT_KEYS / 2) + t / 2) = make_uint2(lo, hi);
-  }
-}
 // Its values as V^T: thread (byte column, 16 tokens) writes two runs of 16 tokens, of entries 16 j + i and 16 j + i + 8.
-__device__ __forceinline__ void operand_values(const uint8_t* __restrict__ raw, const uint32_t* __restrict__ scales, uint8_t* __restrict__ st,
-                                               const Cache4& c, int tid) {
+template <int T>
+__device__ __forceinline__ void operand_values(const uint8_t* __restrict__ raw, uint8_t* __restrict__ st, const Cache4& c, int E, bool deep, int tid) {
   const int columns = c.V / 2;                           // 32 or 64
-#pragma unroll 2
-  for (int u = tid; u < columns * 4; u += 32 * LT_LOADERS) {
+  const uint32_t most = (uint32_t)E * 0x00010001u;
+  for (int u = tid; u < columns * 4; u += T) {
     const int col = u & (columns - 1), t0 = u / columns * 16, j = col / 8, i = col % 8;
     const uint4 vc = *reinterpret_cast<const uint4*>(raw + 36 * c.K + col * C4_TOKENS + t0);
-    const uint4 s0 = *reinterpret_cast<const uint4*>(scales + j * (LT_KEYS / 2) + t0 / 2), s1 = *reinterpret_cast<const uint4*>(scales + j * (LT_KEYS / 2) + t0 / 2 + 4);
-    const uint32_t cw[4] = {vc.x, vc.y, vc.z, vc.w}, sw[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    const uint4 vs = *reinterpret_cast<const uint4*>(raw + 36 * c.K + 32 * c.V + j * C4_TOKENS + t0);
+    const uint4 ve = *reinterpret_cast<const uint4*>(raw + 36 * (c.K + c.V) + C4_TOKENS + t0);
+    const uint32_t cw[4] = {vc.x, vc.y, vc.z, vc.w}, sw[4] = {vs.x, vs.y, vs.z, vs.w}, ew[4] = {ve.x, ve.y, ve.z, ve.w};
     uint8_t* row = st + (16 * j + i) * 128;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {                        // 8 tokens: a chunk of 16 bytes for each of the two entries
@@ -141,8 +124,10 @@ __device__ __forceinline__ void operand_values(const uint8_t* __restrict__ raw, 
         e2m1_pairs(cw[2 * k + q], h);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          lo[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), sw[4 * k + 2 * q + x]);
-          hi[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), sw[4 * k + 2 * q + x]);
+          const uint32_t e = __vminu2(__byte_perm(ew[2 * k + q], 0, x ? 0x4342 : 0x4140), most);
+          const uint32_t scale = scaled_down(e4m3_pair(sw[2 * k + q] >> (16 * x)), most - e, deep);
+          lo[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x5410), scale);
+          hi[2 * q + x] = hmul2(__byte_perm(h[2 * x], h[2 * x + 1], 0x7632), scale);
         }
       }
       const int at = (t0 / 8 + k ^ i) << 4;              // 16 j + i and + 8 are alike modulo 8
@@ -151,38 +136,30 @@ __device__ __forceinline__ void operand_values(const uint8_t* __restrict__ raw, 
     }
   }
 }
-// A row of bf16 queries in its column boxes -> fp16 times 2^(14 - e), e the exponent of its largest magnitude (returned). Chunks are taken in an
-// order that spreads the rows of a warp over the banks.
-__device__ __forceinline__ int operand_query(uint8_t* qs, int q_box, int kcols, int r) {
+// The 64 entries of a query row in one column box: their largest magnitude, and then bf16 -> fp16 times up * up2. Chunks are taken in an order
+// that spreads the rows of a warp over the banks.
+__device__ __forceinline__ float query_most(const uint8_t* row, int r) {
   float most = 0.0f;
-  for (int box = 0; box < kcols; ++box) {
-    const uint8_t* row = qs + box * q_box + r * 128;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint4 v = *reinterpret_cast<const uint4*>(row + (((k + r) & 7) << 4));
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int k = 0; k < 8; ++k) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + (((k + r) & 7) << 4));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
-    }
+    for (int x = 0; x < 4; ++x)
+      most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xffff0000u))));
   }
-  const int e = a4_query_exponent(most);
-  const float up = c4_power((A4_BIAS - e) / 2), up2 = c4_power(A4_BIAS - e - (A4_BIAS - e) / 2);
-  for (int box = 0; box < kcols; ++box) {
-    uint8_t* row = qs + box * q_box + r * 128;
-    uint4 v[8];
+  return most;
+}
+__device__ __forceinline__ void query_to_half(uint8_t* row, int r, float up, float up2) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const uint4*>(row + (((k + r) & 7) << 4));
+  for (int k = 0; k < 8; ++k) {
+    uint4* at = reinterpret_cast<uint4*>(row + (((k + r) & 7) << 4));
+    uint32_t w[4] = {at->x, at->y, at->z, at->w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint32_t w[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        w[x] = pack_half(__uint_as_float(w[x] << 16) * up * up2, __uint_as_float(w[x] & 0xffff0000u) * up * up2);
-      *reinterpret_cast<uint4*>(row + (((k + r) & 7) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int x = 0; x < 4; ++x)
+      w[x] = pack_half(__uint_as_float(w[x] << 16) * up * up2, __uint_as_float(w[x] & 0xffff0000u) * up * up2);
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  return e;
 }
 
 // D (+)= A[tmem] * B[smem]; A: bf16 pairs, one row per lane.
@@ -207,7 +184,7 @@ __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t addr) {
 }
 
 template <int PARTS, bool FOUR = false>
-__global__ void __launch_bounds__(lt_threads(PARTS, FOUR), PARTS == 2 ? 2 : 1)
+__global__ void __launch_bounds__(lt_threads(PARTS), PARTS == 2 ? 2 : 1)
 fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mc,
                              const PagedAttn a, const LatentTc c, const Cache4 c4) {
   constexpr int TCOLS = PARTS == 2 ? 256 : 512;
@@ -254,11 +231,12 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     mbar_init(&sh->q_full, 1);
     mbar_init(&sh->o_done, 1);
     for (int i = 0; i < c.stages; ++i) {
-      mbar_init(&sh->full[i], FOUR ? LT_LOADERS : 1);
+      mbar_init(&sh->full[i], FOUR ? 4 * PARTS : 1);
       mbar_init(&sh->empty[i], 1);
     }
     mbar_init(&sh->raw_full, 1);
-    mbar_init(&sh->q_ready, LT_LOADERS);
+    mbar_init(&sh->raw_empty, 4 * PARTS);
+    mbar_init(&sh->q_ready, PARTS * quarters);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->p_full[i], PARTS * quarters);
@@ -320,7 +298,25 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
                           j < c.kcols ? j * 64 : a.voff + (j - c.kcols) * 64, (b0 * LT_KEYS + nth * box) % a.bs, page);
         }
       }
-      if (!ok && lane == 0) {
+      // FOUR: the raw blocks, one at a time
+      for (; FOUR && i < nb; ++i) {
+        if (i > 0) ok = mbar_wait(&sh->raw_empty, (i - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int in_page = a.bs / LT_KEYS, bytes = c4.bytes();
+        if ((i & 31) == 0) held = (int)a.page_of(seq, min((b0 + i + lane) / in_page, a.nblk - 1));
+        const i64 page = __shfl_sync(0xffffffffu, held, i & 31);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh->raw_full, bytes);
+          bulk_load(raw, c4.p + ((page * a.G + group) * in_page + (b0 + i) % in_page) * bytes, &sh->raw_full, bytes);
+        }
+      }
+      if (FOUR && !ok && lane == 0) {
+        fail();
+        mbar_wait(&sh->q_full, 0);
+        if (i > 0) mbar_wait(&sh->raw_full, (i - 1) & 1);
+      }
+      if (!FOUR && !ok && lane == 0) {
         fail();
         mbar_wait(&sh->q_full, 0);
         for (int k = i > c.stages ? i - c.stages : 0; k < i; ++k) mbar_wait(&sh->full[k % c.stages], (k / c.stages) & 1);
@@ -364,68 +360,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       if (ok) umma_commit(&sh->o_done);
       else fail();
     }
-  } else if (FOUR && warp >= 2 + 4 * PARTS) {
-    // ---- operands from codes: the raw block of the next step is fetched as soon as this one's is used ----
-    const int tid = threadIdx.x - 32 * (2 + 4 * PARTS), bytes = c4.bytes(), in_page = a.bs / LT_KEYS;
-    int held = 0;
-    auto fetch = [&](int i) {                            // the first warp reads the block table for 32 blocks at a time
-      if (warp != 2 + 4 * PARTS) return;
-      if ((i & 31) == 0) held = (int)a.page_of(seq, min((b0 + i + lane) / in_page, a.nblk - 1));
-      const i64 page = __shfl_sync(0xffffffffu, held, i & 31);
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&sh->raw_full, bytes);
-        bulk_load(raw, c4.p + ((page * a.G + group) * in_page + (b0 + i) % in_page) * bytes, &sh->raw_full, bytes);
-      }
-    };
-    if (nb > 0) fetch(0);
-    // a wait that gives up is remembered and the loop goes on, without waits, copies or work: the barrier counts both warps
-    bool ok = nb == 0 || mbar_wait(&sh->q_full, 0);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok && lane == 0) fail();
-    if (ok && nb > 0) {
-      for (int r = tid; r < c.qrows; r += 32 * LT_LOADERS) sh->q_exp[r] = (short)operand_query(qs, q_box, c.kcols, r);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->q_ready);
-    }
-    const int seen_lo = a.first_key(p_first);
-    int E = 0;                                           // the largest value exponent so far
-    for (int i = 0; i < nb; ++i) {
-      const int s = i % c.stages, round = i / c.stages;
-      if (ok) {
-        ok = mbar_wait(&sh->raw_full, i & 1) && (round == 0 || mbar_wait(&sh->empty[s], (round - 1) & 1));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok && lane == 0) fail();
-      }
-      if (ok) {
-        // exponents of the tokens that some row of the tile sees
-        unsigned k_most = 0, v_most = 0, k_least = 255, v_least = 255;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int t = lane + 32 * h;
-          const i64 key = (i64)(b0 + i) * LT_KEYS + t;
-          if (key < seen_lo || key > p_last) continue;
-          const unsigned ke = raw[c4.key_exp(t)], ve = raw[c4.value_exp(t)];
-          k_most = max(k_most, ke), v_most = max(v_most, ve), k_least = min(k_least, ke), v_least = min(v_least, ve);
-        }
-        k_most = __reduce_max_sync(0xffffffffu, k_most), k_least = __reduce_min_sync(0xffffffffu, k_least);
-        E = max(E, (int)__reduce_max_sync(0xffffffffu, v_most)), v_least = __reduce_min_sync(0xffffffffu, v_least);
-        uint8_t* st = ring + s * stage_bytes;
-        operand_scales(raw, sh->scales, c4, E, E > (int)v_least + 14, tid);
-        operand_keys(raw, st, c4, (int)k_most, k_most > k_least + 14, tid);
-        if (tid == 0) sh->exps[s][0] = (int)k_most, sh->exps[s][1] = E;
-      }
-      loaders_barrier();                                 // the scales are there
-      if (ok) {
-        operand_values(raw, sh->scales, ring + s * stage_bytes + c.kcols * LT_KEYS * 128, c4, tid);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->full[s]);
-      }
-      loaders_barrier();                                 // the raw block is read
-      if (ok && i + 1 < nb) fetch(i + 1);
-    }
-  } else if ((warp & 3) < quarters) {
+  } else if (FOUR || (warp & 3) < quarters) {
     // ---- softmax. A wait that gives up is remembered and the loop goes on (the quarter's barriers count every warp) ----
     constexpr int KW = LT_KEYS / PARTS;
     const int quarter = warp & 3, part = (warp - 2) >> 2, r = quarter * 32 + lane;
@@ -440,16 +375,67 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     float den = a.sink && blockIdx.y == 0 && part == 0 ? UNIT : 0.0f;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
-    float row_scale = scale;
-    int E = 0;
-    if (FOUR && nb > 0) {
-      ok = mbar_wait(&sh->q_ready, 0);
+    // ---- FOUR: the operands of a block ----
+    const bool used = (warp & 3) < quarters;             // the others have no queries and only help with the operands
+    const int seen_lo = a.first_key(p_first);
+    int E = 0, k_exp = 0, v_exp = 0, k_exp_next = 0;     // of the accumulator; of this block's keys and values, and of the next one's
+    auto operands = [&](int i) {
+      if (ok) ok = mbar_wait(&sh->raw_full, i & 1) && (i < 2 || mbar_wait(&sh->s_full[i & 1], ((i >> 1) - 1) & 1));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      // exponents of the tokens that some row of the tile sees
+      unsigned k_most = 0, v_most = 0, k_least = 255, v_least = 255;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int t = lane + 32 * h;
+        const i64 key = (i64)(b0 + i) * LT_KEYS + t;
+        if (key < seen_lo || key > p_last) continue;
+        const unsigned ke = raw[c4.key_exp(t)], ve = raw[c4.value_exp(t)];
+        k_most = max(k_most, ke), v_most = max(v_most, ve), k_least = min(k_least, ke), v_least = min(v_least, ve);
+      }
+      k_exp_next = (int)__reduce_max_sync(0xffffffffu, k_most), k_least = __reduce_min_sync(0xffffffffu, k_least);
+      v_exp = max(v_exp, (int)__reduce_max_sync(0xffffffffu, v_most)), v_least = __reduce_min_sync(0xffffffffu, v_least);
+      uint8_t* st = ring + i % c.stages * stage_bytes;
+      operand_keys<128 * PARTS>(raw, st, c4, k_exp_next, k_exp_next > (int)k_least + 14, threadIdx.x - 64);
+      if (i >= 2) ok = mbar_wait(&sh->pv_done[i & 1], ((i >> 1) - 1) & 1);             // the values of block i - 2 are used
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      operand_values<128 * PARTS>(raw, st + c.kcols * LT_KEYS * 128, c4, v_exp, v_exp > (int)v_least + 14, threadIdx.x - 64);
+      fence_proxy_async_smem();
       __syncwarp();
-      const int back = ok ? sh->q_exp[r < c.qrows ? r : 0] - A4_BIAS : 0;
-      row_scale = scale * c4_power(back / 2) * c4_power(back - back / 2);
+      if (lane == 0) {
+        mbar_arrive(&sh->full[i % c.stages]);
+        mbar_arrive(&sh->raw_empty);
+      }
+    };
+    float row_scale = scale;
+    int v_exp_now = 0;
+    if (FOUR && nb > 0) {
+      if (used) {
+        ok = mbar_wait(&sh->q_full, 0);
+        float most = 0.0f;
+        for (int box = part; ok && r < c.qrows && box < c.kcols; box += PARTS) most = fmaxf(most, query_most(qs + box * q_box + r * 128, r));
+        sh->row_max[0][part][r] = most;
+        quarter_barrier<PARTS>(quarter);
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) most = fmaxf(most, sh->row_max[0][k][r]);
+        const int e = a4_query_exponent(most), back = e - A4_BIAS;
+        const float up = c4_power(-back / 2), up2 = c4_power(-back - -back / 2);
+        for (int box = part; ok && r < c.qrows && box < c.kcols; box += PARTS) query_to_half(qs + box * q_box + r * 128, r, up, up2);
+        row_scale = scale * c4_power(back / 2) * c4_power(back - back / 2);
+        ok = __all_sync(0xffffffffu, ok);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&sh->q_ready);
+        quarter_barrier<PARTS>(quarter);                   // row_max is used again
+      }
+      operands(0);
+      k_exp = k_exp_next, v_exp_now = v_exp;
     }
     for (int i = 0; i < nb; ++i) {
       const int buf = i & 1;
+      if (FOUR && i + 1 < nb) operands(i + 1);
+      if (FOUR && !used) continue;
       ok = ok && mbar_wait(&sh->s_full[buf], (i >> 1) & 1);
       __syncwarp();
       tc_fence_after();
@@ -458,13 +444,11 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       for (int k = 0; k < KW; k += 16) tmem_ld16(tmem + lanes + buf * LT_KEYS + part * KW + k, *reinterpret_cast<uint32_t(*)[16]>(u + k));
       tmem_ld_wait();
       float f = 1.0f;
-      if (FOUR && ok) {
-        const int stage = i % c.stages;
-        ok = mbar_wait(&sh->full[stage], (i / c.stages) & 1);            // long done: orders the exponents
-        const int ek = sh->exps[stage][0], ev = sh->exps[stage][1];
-        scale = row_scale * c4_power(ek - 127);
-        if (ev != E && E != 0) f = c4_power(max(E - ev, -126));
-        E = ev;
+      if (FOUR) {
+        scale = row_scale * c4_power(k_exp - 127);
+        if (v_exp_now != E && E != 0) f = c4_power(max(E - v_exp_now, -126));
+        E = v_exp_now;
+        k_exp = k_exp_next, v_exp_now = v_exp;
       }
       const int k0 = (b0 + i) * LT_KEYS + part * KW;
       float s[KW], mx = -INFINITY;
@@ -543,7 +527,8 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       const i64 n = (i64)a.M * a.H * a.G, at = (i64)token * a.H * a.G + head;
       // outputs in units of 1: of the weights where a kernel behind joins parts
       const float units = FOUR && E != 0 ? c4_power(max(E - 127, -126)) : 1.0f;
-      const float inv = c.splits == 1 ? units / den : units / UNIT;
+      float inv = c.splits == 1 ? units / den : units / UNIT;
+      if (FOUR && c.splits == 1 && den == 0.0f) inv = 0.0f;                // a row that sees nothing
       float* acc = c.part + (blockIdx.y * n + at) * a.R + v0;
       bf16* out = static_cast<bf16*>(a.out) + token * a.out_tok + head * a.out_head + v0;
       for (int q = part * 16; q < vn; q += 16 * PARTS) {

@@ -386,6 +386,7 @@ int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, voi
   const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared<true>) + 16 + c4.bytes();
   c.stages = (LT_PAIR_SMEM - fixed) / (c.cols * LT_KEYS * 128);
   if (c.stages > LT_MAX_STAGES) c.stages = LT_MAX_STAGES;
+  if (c.stages < 2) return BX_ELIMIT;                                    // a block's operands are made while the one before it is used
   c.row_blocks = ceil_div(rows, 128);
   c.vsplit = 1;
   c.splits = 1;
@@ -400,7 +401,7 @@ int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, voi
   c.part = static_cast<float*>(scratch);
   CUtensorMap mq;
   if (!make_map_bf16(&mq, a.q, a.W, (i64)a.M * a.H, a.G, a.ldq, (i64)a.M * a.H * a.ldq, c.qrows, 1)) return BX_ELAUNCH;
-  const int rc = launch_chained(fl_paged_attention_tc_kernel<2, true>, dim3(a.ntiles, c.splits, c.row_blocks * a.G), lt_threads(2, true),
+  const int rc = launch_chained(fl_paged_attention_tc_kernel<2, true>, dim3(a.ntiles, c.splits, c.row_blocks * a.G), lt_threads(2),
                                 fixed + c.stages * c.cols * LT_KEYS * 128, st, 0, mq, mq, a, c, c4);
   if (rc != BX_OK || c.splits == 1) return rc;
   // it writes every row; those of short tiles get what is theirs from the kernel behind it
