@@ -97,7 +97,8 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
 //   keys     s = 2^e_k (code scale . q) / sqrt(d); the query row is held in fp16 times a power of two that brings its largest entry to
 //            2^14, so bf16 entries down to 2^-31 of that are exact
 //   values   w = e^(s - max) 2^(e_v - E) 2^14 in fp16 (11 bits; the sum of the weights is of the unrounded ones), E the largest exponent of the
-//            values so far: like the running maximum, the accumulators follow it when it grows
+//            values that the row has seen: like the running maximum, the accumulators follow it when it grows. (The rows of one token see
+//            the same; where a tile has several, a row has its own E, so that no later token costs an earlier one its digits.)
 // A transposed 8x8 register exchange (movmatrix) turns P into the second product's operand: nothing goes through shared memory but the blocks.
 //
 // A tile belongs to one warp (CTAs of one: many tiles), to the W = 4 warps of a CTA, or to a cluster of those (few tiles). A warp takes every
@@ -165,7 +166,8 @@ __host__ __device__ constexpr int a4_ring_bytes() {
   return ring > out ? ring : out;
 }
 
-template <int K, int V, int NT, int W>
+// TILES: of one token or several; else single tokens.
+template <int K, int V, int NT, int W, bool TILES>
 __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_kernel(const PagedAttn a, const Cache4 c, int max_rows) {
   constexpr int BYTES = a4_block_bytes<K, V>(), KS = K / 16, KW = K / 32, ROWS = 8 * NT;
   extern __shared__ __align__(128) uint8_t a4_raw[];
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
   const int tile = blockIdx.x >> (__ffs(ctas) - 1), group = blockIdx.y;
   int tok0, ntok;
   i64 seq;
-  if (a.tiles) {
+  if constexpr (TILES) {
     const int* t = a.tiles + (i64)tile * 3;
     seq = t[0], tok0 = t[1], ntok = t[2];
   } else {
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
     seq = a.seq[tok0];
   }
   const int row0 = blockIdx.z * ROWS, rows = min(ROWS, ntok * a.H - row0);
-  if (rows <= 0 || a.tiles && ntok * a.H > max_rows) return;             // all CTAs of the cluster alike; taller tiles are another kernel's
+  if (rows <= 0 || TILES && ntok * a.H > max_rows) return;             // all CTAs of the cluster alike; taller tiles are another kernel's
   const i64 limit = (i64)a.nblk * a.bs - 1;
   // what depends on nothing but the tile is asked for ahead of the chain position, page, block
   uint32_t q[NT][KS][2];
@@ -284,11 +286,11 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
 
   float out[V / 16][NT][4] = {};                           // entries 16 j + gid (+ 8) of rows 2 tig (+ 1)
   float top[NT][2], den[NT][2];
-  int E = 0;
+  int E[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) top[t][h] = -INFINITY, den[t][h] = 0.0f;
+    for (int h = 0; h < 2; ++h) top[t][h] = -INFINITY, den[t][h] = 0.0f, E[t][h] = 0;
 
   for (int i = 0; ok && i < n; ++i) {
     if (!mbar_wait(&sh->full[warp][i % A4_STAGES], (i / A4_STAGES) & 1)) ok = false;
@@ -351,14 +353,43 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
       }
     }
     uint32_t big = __vmaxu2(__vmaxu2(ve[0], ve[1]), __vmaxu2(ve[2], ve[3]));
-    int e_new = max(E, (int)max(big & 0xffffu, big >> 16));
+    int e_new = (int)max(big & 0xffffu, big >> 16);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, o));
 
     // ---- the running maximum ----
-    bool grows = e_new > E;
-    const float f_e = E == 0 ? 0.0f : c4_power(max(E - e_new, -126));
+    bool grows = false;
     float f[NT][2];
+    if constexpr (TILES) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int e = e_new;
+          if (edge) {
+            e = 0;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+              const int key = k0 + tok + 2 * x;
+              if (key >= row_lo[t][h] && key <= row_hi[t][h]) e = max(e, (int)(x % 2 ? ve[x / 2] >> 16 : ve[x / 2] & 0xffffu));
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+          }
+          e = max(e, E[t][h]);
+          grows |= e > E[t][h];
+          f[t][h] = E[t][h] == 0 ? 0.0f : c4_power(max(E[t][h] - e, -126));
+          E[t][h] = e;
+        }
+    } else {
+      e_new = max(e_new, E[0][0]);
+      grows = e_new > E[0][0];
+      const float f_e = E[0][0] == 0 ? 0.0f : c4_power(max(E[0][0] - e_new, -126));
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) f[t][h] = f_e, E[t][h] = e_new;
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -378,7 +409,6 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
           }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        f[t][h] = f_e;
         if (m > top[t][h]) {
           const float g = a4_exp2(top[t][h] - m);          // 0 for the first keys
           f[t][h] *= g;
@@ -387,7 +417,6 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
           grows = true;
         }
       }
-    E = e_new;
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
       for (int j = 0; j < V / 16; ++j)
@@ -404,7 +433,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
       float g[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int e = (int)(x ? ve[u] >> 16 : ve[u] & 0xffffu) - E + 127 + A4_BIAS;
+        const int e = (int)(x ? ve[u] >> 16 : ve[u] & 0xffffu) - E[0][0] + 127 + A4_BIAS;
         g[x] = __int_as_float(max(e, 0) << 23);
       }
 #pragma unroll
@@ -417,6 +446,10 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
             const float m = top[t][h] == -INFINITY ? 0.0f : top[t][h];
             w[h] = a4_exp2(s[u][t][2 * x + h] - m);
             den[t][h] += w[h];
+            if constexpr (TILES) {                         // (a key that the row does not see may have a larger exponent)
+              const int e = min((int)(x ? ve[u] >> 16 : ve[u] & 0xffffu) - E[t][h], 0) + 127 + A4_BIAS;
+              g[x] = __int_as_float(max(e, 0) << 23);
+            }
             w[h] *= g[x];
           }
           p[u][t][x] = transposed(pack_half(w[0], w[1]));
@@ -461,7 +494,6 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
   together();                                              // all rings are done with
   const bool dead = sh->abort_flag != 0;
   float* slab = reinterpret_cast<float*>(ring_all);        // [row][V] of the CTA, then (W > 1) of every warp
-  const float unit = E == 0 ? 0.0f : c4_power(max(E - 127 - A4_BIAS, -126));
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -470,6 +502,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
       float m = -INFINITY;
 #pragma unroll
       for (int w = 0; w < W; ++w) m = fmaxf(m, sh->max_[w][r]);
+      const float unit = E[t][h] == 0 ? 0.0f : c4_power(max(E[t][h] - 127 - A4_BIAS, -126));
       const float g = unit * (top[t][h] == -INFINITY ? 0.0f : a4_exp2(top[t][h] - m));
       float* to = slab + ((W > 1 ? warp + 1 : 0) * ROWS + r) * V + gid;
 #pragma unroll

@@ -18,9 +18,12 @@
 // A 4-bit cache (FOUR; fl_cache4.cuh): the softmax warps also make the fp16 operands of the next block in shared memory from its codes,
 // in front of a block's softmax, so that its scores are computed meanwhile. A raw block arrives by one bulk copy; keys become
 // K-major rows as a TMA copy would leave them, values, whose codes lie along the tokens, a K-major V^T. An entry is its code times its
-// scale times 2^(e - E), with E the largest exponent of the block's keys (it goes into the scores), or of the values so far (the
-// accumulator is rescaled when it grows): exact for rows within 2^14 of the largest one, off by 2^-36 of that one's largest entry
-// beyond. The queries are turned to fp16 in place, each row times a power of two, and weights are held times 2^6. It is for tiles of
+// scale times 2^(e - E), with E the largest exponent of the block's keys (it goes into the scores) or values (it goes into the weights,
+// relative to the largest exponent of the values that the row has seen; the accumulator is rescaled when that grows): exact for
+// tokens within 2^14 of the largest one; values beyond are off by 2^-36 of that one's largest entry. A token that only some rows see must not cost
+// the others their digits, nor a large key the scores of small ones: blocks where that could be have operands without the powers of two,
+// which then go into every score and weight on its own.
+// The queries are turned to fp16 in place, each row times a power of two, and weights are held times 2^6. It is for tiles of
 // many query rows, which share that work; short tiles have the kernel of fl_attention4.cuh, and each of the two leaves the
 // other's tiles alone. (Two or four warps of their own for the operands were slower: they were a chain of latencies of 4200 cycles a
 // block, where eight warps with other work beside it take turns.)
@@ -28,6 +31,8 @@
 
 #include "fl_attention4.cuh"
 #include "fl_gemm.cuh"
+
+#include <type_traits>
 
 namespace bxf {
 
@@ -79,10 +84,10 @@ __device__ __forceinline__ uint32_t scaled_down(uint32_t scale, uint32_t u, bool
 }
 
 // One block's keys, by T threads: thread (row, 32 entries) writes four chunks of 16 bytes where a 128-byte-swizzled copy would put
-// them. deep: some row is more than 2^14 below E. What is read comes first: a load is not moved in front of a store that might
-// be to the same place.
+// them. E = 0: without the powers of two; else no row that is seen is more than 2^14 below E. What is read comes first: a load is not
+// moved in front of a store that might be to the same place.
 template <int T>
-__device__ __forceinline__ void operand_keys(const uint8_t* __restrict__ raw, uint8_t* __restrict__ st, const Cache4& c, int E, bool deep, int tid) {
+__device__ __forceinline__ void operand_keys(const uint8_t* __restrict__ raw, uint8_t* __restrict__ st, const Cache4& c, int E, int tid) {
   const int r = tid % LT_KEYS;
   const uint32_t down = (E - min((int)raw[c.key_exp(r)], E)) * 0x00010001u;
   for (int part = tid / LT_KEYS; part < c.K / 32; part += T / LT_KEYS) {
@@ -92,7 +97,7 @@ __device__ __forceinline__ void operand_keys(const uint8_t* __restrict__ raw, ui
 #pragma unroll
     for (int j = 0; j < 2; ++j) scale[j] = (raw[c.key_scale(r, part * 2 + j)] & 127) * 0x0101u;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) scale[j] = scaled_down(e4m3_pair(scale[j]), down, deep);
+    for (int j = 0; j < 2; ++j) scale[j] = scaled_down(e4m3_pair(scale[j]), down, false);
     uint8_t* row = st + part / 2 * (LT_KEYS * 128) + r * 128;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -103,7 +108,8 @@ __device__ __forceinline__ void operand_keys(const uint8_t* __restrict__ raw, ui
     }
   }
 }
-// Its values as V^T: thread (byte column, 16 tokens) writes two runs of 16 tokens, of entries 16 j + i and 16 j + i + 8.
+// Its values as V^T: thread (byte column, 16 tokens) writes two runs of 16 tokens, of entries 16 j + i and 16 j + i + 8. deep: some row is
+// more than 2^14 below E.
 template <int T>
 __device__ __forceinline__ void operand_values(const uint8_t* __restrict__ raw, uint8_t* __restrict__ st, const Cache4& c, int E, bool deep, int tid) {
   const int columns = c.V / 2;                           // 32 or 64
@@ -196,7 +202,8 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
   using Shared = LatentShared<FOUR>;
   static_assert(PARTS <= Shared::SHARE, "threads of a row");
   Shared* sh = reinterpret_cast<Shared*>(ring + c.stages * stage_bytes);
-  uint8_t* raw = reinterpret_cast<uint8_t*>(sh) + (sizeof(Shared) + 15) / 16 * 16;           // FOUR: a block as it is in the cache
+  uint8_t* raw = reinterpret_cast<uint8_t*>(sh) + (sizeof(Shared) + 15) / 16 * 16;           // FOUR: a block as it is in the cache, and
+  uint8_t* exps = raw + c4.bytes();                      // the exponents [parity of the block][keys, values][64] of blocks without them
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   wait_previous();
@@ -377,8 +384,13 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     bool ok = true;
     // ---- FOUR: the operands of a block ----
     const bool used = (warp & 3) < quarters;             // the others have no queries and only help with the operands
-    const int seen_lo = a.first_key(p_first);
-    int E = 0, k_exp = 0, v_exp = 0, k_exp_next = 0;     // of the accumulator; of this block's keys and values, and of the next one's
+    // keys that some row sees, that every row sees
+    const int seen_lo = a.first_key(p_first), seen_hi = (int)p_last, whole_lo = a.first_key(p_last), whole_hi = (int)p_first;
+    int E = 0;                                           // of the accumulator: the largest of the values that the row has seen
+    // Of the keys and values of this block, and of the next one; keys' 0: the block's operands are without the powers of two. Those of values
+    // stay as they were from block to block while that costs at most FEW bits.
+    constexpr int FEW = 4;
+    int k_exp = 0, v_exp = 0, k_exp_next = 0, v_exp_next = 0;
     auto operands = [&](int i) {
       if (ok) ok = mbar_wait(&sh->raw_full, i & 1) && (i < 2 || mbar_wait(&sh->s_full[i & 1], ((i >> 1) - 1) & 1));
       ok = __all_sync(0xffffffffu, ok);
@@ -388,19 +400,25 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int t = lane + 32 * h;
-        const i64 key = (i64)(b0 + i) * LT_KEYS + t;
-        if (key < seen_lo || key > p_last) continue;
+        const int key = (b0 + i) * LT_KEYS + t;
+        if (key < seen_lo || key > seen_hi) continue;
         const unsigned ke = raw[c4.key_exp(t)], ve = raw[c4.value_exp(t)];
         k_most = max(k_most, ke), v_most = max(v_most, ve), k_least = min(k_least, ke), v_least = min(v_least, ve);
       }
       k_exp_next = (int)__reduce_max_sync(0xffffffffu, k_most), k_least = __reduce_min_sync(0xffffffffu, k_least);
-      v_exp = max(v_exp, (int)__reduce_max_sync(0xffffffffu, v_most)), v_least = __reduce_min_sync(0xffffffffu, v_least);
+      v_most = __reduce_max_sync(0xffffffffu, v_most), v_least = __reduce_min_sync(0xffffffffu, v_least);
+      const int first = (b0 + i) * LT_KEYS;
+      if (k_exp_next > (int)k_least + 14 || v_most > v_least + FEW && (first < whole_lo || first + LT_KEYS - 1 > whole_hi)) k_exp_next = 0;
+      else if ((int)v_most > v_exp_next || v_exp_next > (int)v_least + FEW) v_exp_next = (int)v_most;
       uint8_t* st = ring + i % c.stages * stage_bytes;
-      operand_keys<128 * PARTS>(raw, st, c4, k_exp_next, k_exp_next > (int)k_least + 14, threadIdx.x - 64);
+      operand_keys<128 * PARTS>(raw, st, c4, k_exp_next, threadIdx.x - 64);
       if (i >= 2) ok = mbar_wait(&sh->pv_done[i & 1], ((i >> 1) - 1) & 1);             // the values of block i - 2 are used
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
-      operand_values<128 * PARTS>(raw, st + c.kcols * LT_KEYS * 128, c4, v_exp, v_exp > (int)v_least + 14, threadIdx.x - 64);
+      operand_values<128 * PARTS>(raw, st + c.kcols * LT_KEYS * 128, c4, k_exp_next ? v_exp_next : 0, k_exp_next && v_most > v_least + 14,
+                                  threadIdx.x - 64);
+      if (k_exp_next == 0 && warp == 2)                          // (block i - 2 is done with: its values are used)
+        *reinterpret_cast<uint32_t*>(exps + (i & 1) * 2 * C4_TOKENS + 4 * lane) = *reinterpret_cast<const uint32_t*>(raw + 36 * (c4.K + c4.V) + 4 * lane);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -409,7 +427,6 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       }
     };
     float row_scale = scale;
-    int v_exp_now = 0;
     if (FOUR && nb > 0) {
       if (used) {
         ok = mbar_wait(&sh->q_full, 0);
@@ -430,12 +447,13 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         quarter_barrier<PARTS>(quarter);                   // row_max is used again
       }
       operands(0);
-      k_exp = k_exp_next, v_exp_now = v_exp;
+      k_exp = k_exp_next, v_exp = v_exp_next;
     }
-    for (int i = 0; i < nb; ++i) {
+    // own (FOUR): the block's operands are without the powers of two, or its values' is below E; the weights take them. Seldom so, and kept out
+    // of the usual case, which is a chain of latencies (394 against 382 us for four prompts of 2048 tokens).
+    auto softmax = [&](int i, auto own) {
+      constexpr bool OWN = decltype(own)::value;
       const int buf = i & 1;
-      if (FOUR && i + 1 < nb) operands(i + 1);
-      if (FOUR && !used) continue;
       ok = ok && mbar_wait(&sh->s_full[buf], (i >> 1) & 1);
       __syncwarp();
       tc_fence_after();
@@ -444,15 +462,18 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       for (int k = 0; k < KW; k += 16) tmem_ld16(tmem + lanes + buf * LT_KEYS + part * KW + k, *reinterpret_cast<uint32_t(*)[16]>(u + k));
       tmem_ld_wait();
       float f = 1.0f;
-      if (FOUR) {
-        scale = row_scale * c4_power(k_exp - 127);
-        if (v_exp_now != E && E != 0) f = c4_power(max(E - v_exp_now, -126));
-        E = v_exp_now;
-        k_exp = k_exp_next, v_exp_now = v_exp;
-      }
+      const bool bare = OWN && k_exp == 0;
+      if (FOUR) scale = row_scale * c4_power(max(k_exp, 1) - 127);
       const int k0 = (b0 + i) * LT_KEYS + part * KW;
+      const uint8_t* block_exps = exps + buf * 2 * C4_TOKENS;
       float s[KW], mx = -INFINITY;
-      if (k0 >= lo && k0 + KW - 1 <= hi) {
+      if (bare) {
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+          s[k] = k0 + k >= lo && k0 + k <= hi ? __uint_as_float(u[k]) * (row_scale * c4_power(block_exps[part * KW + k] - 127)) : -INFINITY;
+          mx = fmaxf(mx, s[k]);
+        }
+      } else if (k0 >= lo && k0 + KW - 1 <= hi) {
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
           s[k] = __uint_as_float(u[k]) * scale;
@@ -471,6 +492,18 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < PARTS; ++k) mx = fmaxf(mx, sh->row_max[buf][k][r]);
+      if (FOUR && k0 - part * KW <= hi && k0 - part * KW + LT_KEYS > lo) {       // the row sees some of the block
+        int e = v_exp;
+        if (bare) {
+          e = 0;
+          for (int k = 0; k < LT_KEYS; ++k)
+            if (k0 - part * KW + k >= lo && k0 - part * KW + k <= hi) e = max(e, (int)block_exps[C4_TOKENS + k]);
+        }
+        if (e > E) {
+          if (E != 0) f = c4_power(max(E - e, -126));
+          E = e;
+        }
+      }
       float g = 1.0f;
       if (mx > ref + LT_GROWTH || ref == -INFINITY) {
         g = ref == -INFINITY ? 0.0f : exp2_fast(ref - mx);
@@ -504,6 +537,12 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         d1 += e1;
         w[k] = FOUR ? pack_half(e0, e1) : pack_bf16(e0, e1);
       }
+      if constexpr (OWN) {
+        const uint8_t* e = block_exps + C4_TOKENS + part * KW;
+#pragma unroll
+        for (int k = 0; k < KW / 2; ++k)
+          w[k] = hmul2(w[k], pack_half(c4_power(max(min((bare ? e[2 * k] : v_exp) - E, 0), -126)), c4_power(max(min((bare ? e[2 * k + 1] : v_exp) - E, 0), -126))));
+      }
       den += d0 + d1;
 #pragma unroll
       for (int k = 0; k < KW / 2; k += 8)
@@ -512,6 +551,16 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->p_full[buf]);
+    };
+    for (int i = 0; i < nb; ++i) {
+      if (FOUR && i + 1 < nb) operands(i + 1);
+      if (!FOUR) {
+        softmax(i, std::false_type{});
+      } else if (used) {
+        if (__any_sync(0xffffffffu, k_exp == 0 || v_exp < E)) softmax(i, std::true_type{});
+        else softmax(i, std::false_type{});
+        k_exp = k_exp_next, v_exp = v_exp_next;
+      }
     }
     if (nb > 0) ok = ok && mbar_wait(&sh->o_done, 0);
     ok = __all_sync(0xffffffffu, ok);

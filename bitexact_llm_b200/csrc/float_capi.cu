@@ -342,16 +342,17 @@ Share4 attention4_share(i64 tiles, i64 blocks, int per_sm) {
   return {4, c};
 }
 
-template <int K, int V, int NT, int W>
+template <int K, int V, int NT, int W, bool TILES>
 int launch_attention4(const PagedAttn& a, const Cache4& c, int most, dim3 grid, int cluster, cudaStream_t st) {
   constexpr int smem = a4_ring_bytes<K, V, NT, W>() + sizeof(A4Shared<W>);
+  constexpr auto kernel = fl_attention4_kernel<K, V, NT, W, TILES>;
   static PerDevice configured;
   if (once_per_device(configured, [] {
-        const cudaError_t e = cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        return e != cudaSuccess ? e : cudaFuncSetAttribute(fl_attention4_kernel<K, V, NT, W>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       }) != BX_OK)
     return BX_ELAUNCH;
-  return launch_chained(fl_attention4_kernel<K, V, NT, W>, grid, 32 * W, smem, st, cluster, a, c, most);
+  return launch_chained(kernel, grid, 32 * W, smem, st, cluster, a, c, most);
 }
 
 template <int K, int V, int NT>
@@ -361,7 +362,9 @@ int launch_attention4(const PagedAttn& a, const Cache4& c, int most, cudaStream_
   const i64 table = (i64)a.nblk * a.bs, seen = a.window > 0 && a.window < table ? a.window + C4_TOKENS : table;
   const Share4 s = attention4_share((i64)n * a.G * z, (seen + C4_TOKENS - 1) / C4_TOKENS, NT == 2 ? 2 : K + V == 128 ? 4 : 3);
   const dim3 grid((unsigned)n * s.ctas, a.G, z);
-  return s.warps == 1 ? launch_attention4<K, V, NT, 1>(a, c, most, grid, 1, st) : launch_attention4<K, V, NT, 4>(a, c, most, grid, s.ctas, st);
+  if (a.tiles)
+    return s.warps == 1 ? launch_attention4<K, V, NT, 1, true>(a, c, most, grid, 1, st) : launch_attention4<K, V, NT, 4, true>(a, c, most, grid, s.ctas, st);
+  return s.warps == 1 ? launch_attention4<K, V, NT, 1, false>(a, c, most, grid, 1, st) : launch_attention4<K, V, NT, 4, false>(a, c, most, grid, s.ctas, st);
 }
 
 template <int NT>
@@ -383,7 +386,7 @@ int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, voi
   c.min_rows = min_rows;
   const int tokens = bxf_latent_attention_tile(a.H), rows = tokens * a.H;
   c.qrows = rows >= 128 ? 128 : ceil_div(rows, 8) * 8;
-  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared<true>) + 16 + c4.bytes();
+  const int fixed = 1024 + c.kcols * c.qrows * 128 + (int)sizeof(LatentShared<true>) + 16 + c4.bytes() + 4 * C4_TOKENS;
   c.stages = (LT_PAIR_SMEM - fixed) / (c.cols * LT_KEYS * 128);
   if (c.stages > LT_MAX_STAGES) c.stages = LT_MAX_STAGES;
   if (c.stages < 2) return BX_ELIMIT;                                    // a block's operands are made while the one before it is used

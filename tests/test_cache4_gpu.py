@@ -272,6 +272,31 @@ def test_large_and_small_magnitudes(variant, dtype):
         close(got, want.expand(90, -1), big, dtype)
 
 
+@pytest.mark.parametrize("dtype,variant", [("bfloat16", 0), ("bfloat16", 1), ("bfloat16", 2), ("float32", 0)])
+@pytest.mark.parametrize("per", [1, 4])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("keys,values", [(1.0, 1e25), (1e20, 1.0), (1e20, 1e25)])
+def test_large_tokens_cost_nothing_to_rows_that_do_not_see_them(keys, values, window, per, dtype, variant):
+    """Tiles, tall ones and short ones, in which some tokens are larger by powers that no number of 16 bits spans: rows in front of them,
+    or behind them by more than the window, keep the accuracy of their own values."""
+    from bitexact_llm_b200.hybrid import ops
+    sp, T, n, G, before = spec(2 * per, 2, 64, 128, window), getattr(torch, dtype), 300, 2, 70
+    big = [100, 163, 164, 250, 299]
+    k, v = rows(n, G, 64, dtype, 5).float(), rows(n, G, 128, dtype, 6).float()
+    k[big] *= keys
+    v[big] *= values
+    cache, slot = ops.gqa_cache4(sp, 6, 64, "cuda"), torch.arange(n).cuda() + 64
+    ops.gqa_store4(k.to(T).cuda(), v.to(T).cuda(), slot, cache)
+    held = [tuple(x.double().cpu() for x in ops.gqa_read4(cache, sp, slot, torch.float32))]
+    bt, M = torch.arange(1, 6, dtype=torch.int32).cuda()[None], n - before
+    q = torch.randn(G, M, per, 64, generator=torch.Generator().manual_seed(7)).to(T)
+    seq, pos = torch.zeros(M, dtype=torch.long).cuda(), torch.arange(before, n).cuda()
+    want, size = attention(q, sp, seq, pos, held, None)
+    for tall in (128 // per, 8 // per):
+        t = torch.tensor([[0, i, min(tall, M - i)] for i in range(0, M, tall)], dtype=torch.int32).cuda()
+        close(ops.gqa_attention4(q.cuda(), sp, cache, bt, seq, pos, None, t, variant)[:, : 2 * per * 128], want, size, dtype)
+
+
 @pytest.mark.parametrize("variant", VARIANTS)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_what_is_not_a_number_stays_with_those_who_see_it(dtype, variant):
