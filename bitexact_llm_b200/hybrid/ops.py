@@ -265,7 +265,9 @@ def gqa_read4(cache, spec, slot, dtype):
 
 
 def gqa_attention4(q, spec, cache, bt, seq, pos, sink, tiles=None, variant=0):
-    """`gqa_attention` over a 4-bit cache: q T [kv_heads, M, heads per group, ldq] -> T [M, pad8(heads vdim)]."""
+    """`gqa_attention` over a 4-bit cache: q T [kv_heads, M, heads per group, ldq] -> T [M, pad8(heads vdim)]. With tiles (of at most
+    `bxf_latent_attention_tile(heads per group)` tokens each, positions ascending) the rows that are in one are written. bf16 outputs are off by at
+    most 2^-11 of the largest value that the row sees and their own rounding."""
     G, M, per, ldq = q.shape
     H, dim, vdim = spec.heads, spec.dim, spec.vdim
     if cache.shape[1] != G or G * per != H or ldq < dim or q.dtype not in (torch.bfloat16, torch.float32) or not q.is_contiguous():
