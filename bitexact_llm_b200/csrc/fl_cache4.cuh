@@ -96,7 +96,7 @@ __device__ __forceinline__ int c4_scale_for(float most) {
 // remainder, is the correctly rounded one, and exact where it is a tie. The entries of bf16 rows come no nearer to a tie without being
 // one than 2^-12 of it; those of 32-bit rows may round to one, and are set beside it by the sign of what remains.
 template <class T>
-__device__ __forceinline__ int c4_codes(const float (&y)[4], float step, float inv) {
+__device__ __forceinline__ uint32_t c4_codes(const float (&y)[4], float step, float inv) {
   float q[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -113,42 +113,43 @@ __device__ __forceinline__ int c4_codes(const float (&y)[4], float step, float i
       "cvt.rn.satfinite.e2m1x2.f32 x, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 y, %4, %3;\n\tmov.b32 %0, {x, y, z, z};\n\t}"
       : "=r"(c)
       : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
-  return (int)c;
+  return c;
 }
 
-// A warp's row: lane l holds entries 128 i + 4 l .. + 3, i < N.
+// A row of half a warp: lane l of 16 holds entries 128 i + 8 l .. + 7, i < N, so that two lanes share a block of 16 and its scale.
 template <class T, int N>
 struct C4Row {
-  float x[N][4];
+  float x[N][8];
 
-  __device__ __forceinline__ void load(const T* p, int n, int lane) {
-    const bool wide = (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
+  __device__ __forceinline__ void load(const T* p, int n, int l) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int d = 128 * i + 4 * lane;
-      if (wide && d + 4 <= n) {
+      const int d = 128 * i + 8 * l;
+      if ((at & 15) == 0 && d + 8 <= n) {
         if constexpr (sizeof(T) == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p + d);
-          x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+          const float4 v = *reinterpret_cast<const float4*>(p + d), w = *reinterpret_cast<const float4*>(p + d + 4);
+          x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w, x[i][4] = w.x, x[i][5] = w.y, x[i][6] = w.z, x[i][7] = w.w;
         } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(p + d);
-          x[i][0] = __uint_as_float(v.x << 16), x[i][1] = __uint_as_float(v.x & 0xffff0000u);
-          x[i][2] = __uint_as_float(v.y << 16), x[i][3] = __uint_as_float(v.y & 0xffff0000u);
+          const uint4 v = *reinterpret_cast<const uint4*>(p + d);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[i][2 * k] = __uint_as_float(w[k] << 16), x[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[i][k] = d + k < n ? ld(p + d + k) : 0.0f;
+        for (int k = 0; k < 8; ++k) x[i][k] = d + k < n ? ld(p + d + k) : 0.0f;
       }
     }
   }
   // -> the largest magnitude of the row as bits, which order like the numbers; NaN and infinities are above all of them.
-  __device__ __forceinline__ uint32_t most() const {
+  __device__ __forceinline__ uint32_t most(int lane) const {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) m = max(m, __float_as_uint(x[i][k]) & 0x7fffffffu);
-    return __reduce_max_sync(0xffffffffu, m);
+      for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(x[i][k]) & 0x7fffffffu);
+    return __reduce_max_sync(0xffffu << (lane & 16), m);
   }
   // Entries that are no numbers become 0, those beyond 2^127 that; -> the largest magnitude of the row then.
   __device__ __noinline__ float mend() {
@@ -156,22 +157,27 @@ struct C4Row {
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k) {
         if (!(fabsf(x[i][k]) < INFINITY)) x[i][k] = 0.0f;
         x[i][k] = fminf(fmaxf(x[i][k], -1.7014118e38f), 1.7014118e38f);
         m = fmaxf(m, fabsf(x[i][k]));
       }
-    return warp_max(m);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
   }
-  // Codes of the lane's four entries (4 bits each) and the scale of their block.
-  __device__ __forceinline__ int codes(int i, float unit, int& scale) const {
-    const float y[4] = {x[i][0] * unit, x[i][1] * unit, x[i][2] * unit, x[i][3] * unit};
-    float m = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+  // Codes of the lane's eight entries (4 bits each) and the scale of their block.
+  __device__ __forceinline__ uint32_t codes(int i, float unit, int& scale) const {
+    float y[8], m = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      y[k] = x[i][k] * unit;
+      m = fmaxf(m, fabsf(y[k]));
+    }
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     scale = c4_scale_for<T>(m);
-    const float step = c4_scale(scale);
-    return c4_codes<T>(y, step, step > 0.0f ? __fdividef(1.0f, step) : 0.0f);
+    const float step = c4_scale(scale), inv = step > 0.0f ? __fdividef(1.0f, step) : 0.0f;
+    return c4_codes<T>({y[0], y[1], y[2], y[3]}, step, inv) | c4_codes<T>({y[4], y[5], y[6], y[7]}, step, inv) << 16;
   }
 };
 
@@ -189,17 +195,21 @@ struct Store4 {
   Cache4 c;
 };
 
-constexpr int S4_THREADS = 128;
+__host__ __device__ constexpr int s4_threads(int rows) { return rows < 8 ? 16 * rows : 128; }
 
-// ROWS rows of one head per CTA, a warp per row. Keys go out as they are made (a row is contiguous); the bytes of values lie along the
+// ROWS rows of one head per CTA, half a warp per row. Keys go out as they are made (a row is contiguous); the bytes of values lie along the
 // tokens: with many rows they are put together in shared memory, and 16 (or 4) rows that lie in a run of slots go out as one store.
+// What bounds it is issue, at some 240 instructions for 256 entries of bf16: 8192 rows of 8 heads in 29 us (1.5 TB/s; a warp per row, in which four
+// lanes made the scale of a block, took 42).
 template <class T, int ROWS, int N>
-__global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a) {
-  constexpr int PITCH = ROWS + 4;      // bytes of a value column of the CTA's rows
+__global__ void __launch_bounds__(s4_threads(ROWS)) fl_store4_kernel(const Store4<T> a) {
+  constexpr int PITCH = ROWS + 4, THREADS = s4_threads(ROWS), STEP = THREADS / 16;  // bytes of a value column of the CTA's rows; rows at a time
+  constexpr bool GATHER = ROWS > STEP;
   extern __shared__ __align__(16) uint8_t s4_smem[];
   __shared__ i64 slots[ROWS];
   __shared__ uint8_t* blocks[ROWS];                        // of the rows' tokens; NULL: a row that is left out
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y, row0 = blockIdx.x * ROWS;
+  __shared__ uint32_t in16, in4;                           // rows whose slot follows on from a multiple of 16 (4) of the first of their 16 (4)
+  const int lane = threadIdx.x & 31, l = lane & 15, g = blockIdx.y, row0 = blockIdx.x * ROWS;
   const Cache4& c = a.c;
   launch_next();
   wait_previous();
@@ -207,86 +217,96 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
     const i64 s = row0 + (int)threadIdx.x < a.M ? a.slot[row0 + threadIdx.x] : -1;
     slots[threadIdx.x] = c.has(s) ? s : -1;
     blocks[threadIdx.x] = c.has(s) ? c.block(s, g) : nullptr;
+    if constexpr (GATHER) {
+      static_assert(ROWS == 32, "a warp");
+      const i64 mine = c.has(s) ? s : -1, f16 = __shfl_sync(0xffffffffu, mine, lane & 16), f4 = __shfl_sync(0xffffffffu, mine, lane & 28);
+      const uint32_t b16 = __ballot_sync(0xffffffffu, f16 >= 0 && f16 % 16 == 0 && mine == f16 + (lane & 15));
+      const uint32_t b4 = __ballot_sync(0xffffffffu, f4 >= 0 && f4 % 4 == 0 && mine == f4 + (lane & 3));
+      if (lane == 0) in16 = b16, in4 = b4;
+    }
   }
   __syncthreads();
   const int columns = c.V / 2 + c.V / 16 + 1;              // of value bytes: codes, scales, the exponent
   C4Row<T, N> k, v, k_next, v_next;
+  const i64 m0 = row0 + (int)threadIdx.x / 16;
+  const T *from_k = a.k + m0 * a.k_row + g * a.k_head, *from_v = a.v + m0 * a.v_row + g * a.v_head;
   auto fetch = [&](int r) {
-    if (r >= ROWS || slots[r] < 0) return;
-    const i64 m = row0 + r;
-    k_next.load(a.k + m * a.k_row + g * a.k_head, c.dim, lane);
-    v_next.load(a.v + m * a.v_row + g * a.v_head, c.vdim, lane);
+    if (r >= ROWS) return;
+    const bool live = slots[r] >= 0;                       // (nothing is read of others)
+    k_next.load(from_k, live ? c.dim : 0, l);
+    v_next.load(from_v, live ? c.vdim : 0, l);
+    from_k += STEP * a.k_row, from_v += STEP * a.v_row;
   };
-  fetch(warp);
-  for (int r = warp; r < ROWS; r += S4_THREADS / 32) {
+  fetch(threadIdx.x / 16);
+  for (int r = threadIdx.x / 16; r < ROWS; r += STEP) {    // (STEP divides ROWS: the halves of a warp go together)
     k = k_next, v = v_next;
-    fetch(r + S4_THREADS / 32);
-    if (slots[r] < 0) continue;
-    const int tok = (int)(slots[r] % C4_TOKENS);
+    fetch(r + STEP);
+    const bool live = slots[r] >= 0;
+    if (!__any_sync(0xffffffffu, live)) continue;
+    const int tok = (int)(slots[r] & (C4_TOKENS - 1));
     uint8_t* block = blocks[r];
-    const uint32_t bits_k = k.most(), bits_v = v.most();
+    const uint32_t bits_k = k.most(lane), bits_v = v.most(lane);
     const bool bad = max(bits_k, bits_v) >= 0x7f800000u;
     float most_k = __uint_as_float(bits_k), most_v = __uint_as_float(bits_v);
-    if (max(bits_k, bits_v) > 0x7f000000u) most_k = k.mend(), most_v = v.mend();
+    if (__any_sync(0xffffffffu, max(bits_k, bits_v) > 0x7f000000u)) most_k = k.mend(), most_v = v.mend();
     const int ek = c4_exponent(most_k), ev = c4_exponent(most_v);
     const float uk = c4_power(-ek), uv = bad ? 0.0f : c4_power(-ev);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (128 * i >= c.K) break;
       int scale;
-      const int code = k.codes(i, uk, scale), d = 128 * i + 4 * lane;
-      if (d < c.K) {
-        *reinterpret_cast<uint16_t*>(block + tok * (c.K / 2) + d / 2) = (uint16_t)code;
-        if ((lane & 3) == 0) block[c.key_scale(tok, d / 16)] = bad ? C4_NAN : scale;
+      const uint32_t code = k.codes(i, uk, scale);
+      const int d = 128 * i + 8 * l;
+      if (live && d < c.K) {
+        *reinterpret_cast<uint32_t*>(block + tok * (c.K / 2) + d / 2) = code;
+        if ((l & 1) == 0) block[c.key_scale(tok, d / 16)] = bad ? C4_NAN : scale;
       }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (128 * i >= c.V) break;
       int scale;
-      const int code = v.codes(i, uv, scale), other = __shfl_xor_sync(0xffffffffu, code, 2), d = 128 * i + 4 * lane;
-      if (d < c.V) {
-        const int j = d / 16;
-        if ((lane & 2) == 0) {
+      const uint32_t code = v.codes(i, uv, scale), other = __shfl_xor_sync(0xffffffffu, code, 1);
+      const int d = 128 * i + 8 * l, j = d / 16, odd = l & 1;
+      if (live && d < c.V) {
+        // the pair's 16 entries in 8 bytes, entry q low and q + 8 high: four to each lane, from halves of its and its neighbour's codes
+        uint32_t lo = odd ? other >> 16 : code & 0xffffu, hi = odd ? code >> 16 : other & 0xffffu;
+        lo = (lo | lo << 8) & 0x00ff00ffu, hi = (hi | hi << 8) & 0x00ff00ffu;
+        lo = (lo | lo << 4) & 0x0f0f0f0fu, hi = (hi | hi << 4) & 0x0f0f0f0fu;
+        const uint32_t bytes = lo | hi << 4;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint8_t byte = (code >> (4 * q) & 15) | (other >> (4 * q) & 15) << 4;
-            const int at = (lane & 1) * 4 + q;
-            if (ROWS > 4) s4_smem[(j * 8 + at) * PITCH + r] = byte;
-            else block[c.value_code(tok, j, at)] = byte;
-          }
-        } else if ((lane & 3) == 3) {
-          if (ROWS > 4) s4_smem[(c.V / 2 + j) * PITCH + r] = scale;
+        for (int q = 0; q < 4; ++q) {
+          const uint8_t byte = bytes >> (8 * q);
+          if (GATHER) s4_smem[(j * 8 + odd * 4 + q) * PITCH + r] = byte;
+          else block[c.value_code(tok, j, odd * 4 + q)] = byte;
+        }
+        if (odd) {
+          if (GATHER) s4_smem[(c.V / 2 + j) * PITCH + r] = scale;
           else block[c.value_scale(tok, j)] = scale;
         }
       }
     }
-    if (lane == 0) {
+    if (live && l == 0) {
       block[c.key_exp(tok)] = ek + 127;
-      if (ROWS > 4) s4_smem[(columns - 1) * PITCH + r] = ev + 127;
+      if (GATHER) s4_smem[(columns - 1) * PITCH + r] = ev + 127;
       else block[c.value_exp(tok)] = ev + 127;
     }
   }
-  if (ROWS <= 4) return;
+  if (!GATHER) return;
   __syncthreads();
   // value bytes: [column][token] in the block, columns 64 apart from its codes on, the exponents at their own place
-  for (int i = threadIdx.x; i < columns * (ROWS / 16); i += S4_THREADS) {
+  for (int i = threadIdx.x; i < columns * (ROWS / 16); i += THREADS) {
     const int col = i % columns, r0 = i / columns * 16;
     const uint8_t* from = s4_smem + col * PITCH + r0;
-    const i64 s0 = slots[r0];
     const int place = col < columns - 1 ? 36 * c.K + col * C4_TOKENS : 36 * (c.K + c.V) + C4_TOKENS;
-    auto at = [&](int r) { return blocks[r] + place + (int)(slots[r] % C4_TOKENS); };
-    bool run = s0 >= 0 && s0 % 16 == 0;
-#pragma unroll
-    for (int k = 1; k < 16; ++k) run &= slots[r0 + k] == s0 + k;
+    auto at = [&](int r) { return blocks[r] + place + ((int)slots[r] & (C4_TOKENS - 1)); };
     const uint32_t* w = reinterpret_cast<const uint32_t*>(from);
-    if (run) {
+    if ((in16 >> r0 & 0xffffu) == 0xffffu) {
       *reinterpret_cast<uint4*>(at(r0)) = make_uint4(w[0], w[1], w[2], w[3]);
       continue;
     }
     for (int k = 0; k < 16; k += 4) {
-      const i64 s = slots[r0 + k];
-      if (s >= 0 && s % 4 == 0 && slots[r0 + k + 1] == s + 1 && slots[r0 + k + 2] == s + 2 && slots[r0 + k + 3] == s + 3) {
+      if ((in4 >> (r0 + k) & 15u) == 15u) {
         *reinterpret_cast<uint32_t*>(at(r0 + k)) = w[k / 4];
         continue;
       }
@@ -296,9 +316,10 @@ __global__ void __launch_bounds__(S4_THREADS) fl_store4_kernel(const Store4<T> a
   }
 }
 
-// The entries that the cache holds at `slot`: k T [M][G][dim], v T [M][G][vdim]; slots outside the cache give zeros. A warp per row and
-// head, a lane for four entries (the codes of a key row lie together; a lane's four of a value are four bytes 64 apart).
-constexpr int R4_WARPS = 8;
+// The entries that the cache holds at `slot`: k T [M][G][dim], v T [M][G][vdim]; slots outside the cache give zeros. Half a warp per row and
+// head, a lane for eight entries (of a value: four bytes 64 apart, entries 8 apart in their halves). A CTA has rows of one head: they share the sectors of the
+// values' bytes where their slots are neighbours: 8192 rows of 8 heads in 13 us behind the store, 27 with the heads of a row together.
+constexpr int R4_ROWS = 8;                                 // of a CTA
 
 template <class T>
 __device__ __forceinline__ void c4_put(T* p, int d, int n, const float (&x)[4]) {
@@ -311,39 +332,41 @@ __device__ __forceinline__ void c4_put(T* p, int d, int n, const float (&x)[4]) 
 }
 
 template <class T>
-__global__ void __launch_bounds__(32 * R4_WARPS) fl_read4_kernel(const Cache4 c, const i64* slot, T* k, T* v, i64 rows) {
+__global__ void __launch_bounds__(16 * R4_ROWS) fl_read4_kernel(const Cache4 c, const i64* slot, T* k, T* v, int M) {
   launch_next();
   wait_previous();
-  const uint32_t at = blockIdx.x * R4_WARPS + (threadIdx.x >> 5);          // below 2^31 + 8
-  const int lane = threadIdx.x & 31;
-  if (at >= rows) return;
-  const uint32_t m = at / (uint32_t)c.G;
-  const i64 s = slot[m];
+  const i64 m = (i64)blockIdx.x * R4_ROWS + (threadIdx.x >> 4);
+  const int l = threadIdx.x & 15, g = blockIdx.y;
+  if (m >= M) return;
+  const i64 s = slot[m], at = m * c.G + g;
   const bool in = c.has(s);
-  const int tok = in ? (int)(s % C4_TOKENS) : 0;
-  const uint8_t* b = c.block(in ? s : 0, (int)(at - m * c.G));
+  const int tok = in ? (int)(s & (C4_TOKENS - 1)) : 0;
+  const uint8_t* b = c.block(in ? s : 0, g);
   const float pk = in ? __int_as_float(b[c.key_exp(tok)] << 23) : 0.0f, pv = in ? __int_as_float(b[c.value_exp(tok)] << 23) : 0.0f;
-  auto put = [&](T* to, int d, int n, uint32_t codes, uint32_t scale, float power) {
+  // bytes of two codes each -> their entries, x of the low codes and y of the high ones
+  auto entries = [&](uint32_t codes, uint32_t scale, float power, float (&x)[4], float (&y)[4]) {
     uint32_t h[4];
     e2m1_pairs(codes, h);
     const uint32_t f = e4m3_pair((scale & 127) * 0x0101u);
-    float x[4];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const uint32_t v = hmul2(h[q], f);
-      const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&v));
-      x[2 * q] = in ? w.x * power : 0.0f, x[2 * q + 1] = in ? w.y * power : 0.0f;
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t w = hmul2(h[q], f);
+      const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&w));
+      x[q] = in ? z.x * power : 0.0f, y[q] = in ? z.y * power : 0.0f;
     }
-    c4_put(to, d, n, x);
   };
-  for (int d = 4 * lane; d < c.dim; d += 128)
-    put(k + (i64)at * c.dim, d, c.dim, *reinterpret_cast<const uint16_t*>(b + tok * (c.K / 2) + d / 2) * 0x10001u, b[c.key_scale(tok, d / 16)], pk);
-  for (int d = 4 * lane; d < c.vdim; d += 128) {
+  float x[4], y[4];
+  for (int d = 8 * l; d < c.dim; d += 128) {
+    entries(*reinterpret_cast<const uint32_t*>(b + tok * (c.K / 2) + d / 2), b[c.key_scale(tok, d / 16)], pk, x, y);
+    c4_put(k + at * c.dim, d, c.dim, {x[0], y[0], x[1], y[1]});
+    c4_put(k + at * c.dim, d + 4, c.dim, {x[2], y[2], x[3], y[3]});
+  }
+  for (int d = 16 * (l / 2) + 4 * (l & 1); d < c.vdim; d += 128) {
     const uint8_t* from = b + c.value_code(tok, d / 16, d % 8);
-    const int half = d % 16 / 8 * 4;
-    const uint32_t codes = (from[0] >> half & 15) | (from[C4_TOKENS] >> half & 15) << 4 | (from[2 * C4_TOKENS] >> half & 15) << 8 |
-                           (from[3 * C4_TOKENS] >> half & 15) << 12;
-    put(v + (i64)at * c.vdim, d, c.vdim, codes, b[c.value_scale(tok, d / 16)], pv);
+    const uint32_t lo = __byte_perm(from[0], from[C4_TOKENS], 0x0040), hi = __byte_perm(from[2 * C4_TOKENS], from[3 * C4_TOKENS], 0x0040);
+    entries(__byte_perm(lo, hi, 0x5410), b[c.value_scale(tok, d / 16)], pv, x, y);
+    c4_put(v + at * c.vdim, d, c.vdim, x);
+    c4_put(v + at * c.vdim, d + 8, c.vdim, y);
   }
 }
 

@@ -304,12 +304,12 @@ Cache4 cache4_of(const void* cache, int kv_heads, int dim, int vdim, int page, i
   return {static_cast<uint8_t*>(const_cast<void*>(cache)), nb, kv_heads, page, dim, vdim, ceil_div(dim, 64) * 64, ceil_div(vdim, 64) * 64};
 }
 
-// Many rows: 32 to a CTA, so that the bytes of their values leave together; few: a CTA for every four.
+// Many rows: 32 to a CTA, so that the bytes of their values leave together; few: a small CTA for every four.
 template <class T, int N>
 int launch_store4(const Store4<T>& a, cudaStream_t st) {
   if (a.M <= 512)
-    return launch_chained(fl_store4_kernel<T, 4, N>, dim3(ceil_div(a.M, 4), a.c.G), S4_THREADS, 0, st, 0, a);
-  return launch_chained(fl_store4_kernel<T, 32, N>, dim3(ceil_div(a.M, 32), a.c.G), S4_THREADS, (a.c.V / 2 + a.c.V / 16 + 1) * 36, st, 0, a);
+    return launch_chained(fl_store4_kernel<T, 4, N>, dim3(ceil_div(a.M, 4), a.c.G), s4_threads(4), 0, st, 0, a);
+  return launch_chained(fl_store4_kernel<T, 32, N>, dim3(ceil_div(a.M, 32), a.c.G), s4_threads(32), (a.c.V / 2 + a.c.V / 16 + 1) * 36, st, 0, a);
 }
 
 template <class T>
@@ -793,13 +793,11 @@ int bxf_gqa_read4(int dtype, const void* cache, int kv_heads, int dim, int vdim,
   if (!slot || !k || !v) return BX_EARG;
   const Cache4 c = cache4_of(cache, kv_heads, dim, vdim, page, nb);
   const i64* slot_ = reinterpret_cast<const i64*>(slot);
-  const i64 rows = (i64)M * kv_heads;
-  if (rows > 0x7fffffffll) return BX_ELIMIT;
-  const dim3 grid((unsigned)((rows + R4_WARPS - 1) / R4_WARPS));
+  const dim3 grid((unsigned)(((i64)M + R4_ROWS - 1) / R4_ROWS), kv_heads);
   cudaStream_t st = stream_of(stream);
   if (dtype == BXF_F32)
-    return launch_chained(fl_read4_kernel<float>, grid, 32 * R4_WARPS, 0, st, 0, c, slot_, static_cast<float*>(k), static_cast<float*>(v), rows);
-  return launch_chained(fl_read4_kernel<bf16>, grid, 32 * R4_WARPS, 0, st, 0, c, slot_, static_cast<bf16*>(k), static_cast<bf16*>(v), rows);
+    return launch_chained(fl_read4_kernel<float>, grid, 16 * R4_ROWS, 0, st, 0, c, slot_, static_cast<float*>(k), static_cast<float*>(v), M);
+  return launch_chained(fl_read4_kernel<bf16>, grid, 16 * R4_ROWS, 0, st, 0, c, slot_, static_cast<bf16*>(k), static_cast<bf16*>(v), M);
 }
 
 int bxf_gqa_attention4(int dtype, const void* q, int64_t ldq, int M, int heads, int kv_heads, int dim, int vdim, const void* cache, int page,
