@@ -159,17 +159,18 @@ __device__ __forceinline__ int a4_query_exponent(float most) {
 
 template <int K, int V>
 __host__ __device__ constexpr int a4_block_bytes() { return 36 * (K + V) + 2 * C4_TOKENS; }
-// The warps' rings; at the end the same memory holds the warps' outputs, rows of V floats.
+// The warps' rings; at the end the same memory holds the warps' outputs, rows of V floats (and 4: the rows that a warp writes at a time lie in
+// different banks).
 template <int K, int V, int NT, int W>
 __host__ __device__ constexpr int a4_ring_bytes() {
-  const int ring = W * A4_STAGES * a4_block_bytes<K, V>(), out = (W > 1 ? W + 1 : 1) * 8 * NT * V * 4;
+  const int ring = W * A4_STAGES * a4_block_bytes<K, V>(), out = (W > 1 ? W + 1 : 1) * 8 * NT * (V + 4) * 4;
   return ring > out ? ring : out;
 }
 
 // TILES: of one token or several; else single tokens.
 template <int K, int V, int NT, int W, bool TILES>
 __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_kernel(const PagedAttn a, const Cache4 c, int max_rows) {
-  constexpr int BYTES = a4_block_bytes<K, V>(), KS = K / 16, KW = K / 32, ROWS = 8 * NT;
+  constexpr int BYTES = a4_block_bytes<K, V>(), KS = K / 16, KW = K / 32, ROWS = 8 * NT, PITCH = V + 4;
   extern __shared__ __align__(128) uint8_t a4_raw[];
   uint8_t* ring_all = a4_raw;
   auto* sh = reinterpret_cast<A4Shared<W>*>(a4_raw + a4_ring_bytes<K, V, NT, W>());
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
       for (int w = 0; w < W; ++w) m = fmaxf(m, sh->max_[w][r]);
       const float unit = E[t][h] == 0 ? 0.0f : c4_power(max(E[t][h] - 127 - A4_BIAS, -126));
       const float g = unit * (top[t][h] == -INFINITY ? 0.0f : a4_exp2(top[t][h] - m));
-      float* to = slab + ((W > 1 ? warp + 1 : 0) * ROWS + r) * V + gid;
+      float* to = slab + ((W > 1 ? warp + 1 : 0) * ROWS + r) * PITCH + gid;
 #pragma unroll
       for (int j = 0; j < V / 16; ++j) {
         to[16 * j] = out[j][t][h] * g;
@@ -520,11 +521,14 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
     }
   together();
   if constexpr (W > 1) {
-    for (int i = threadIdx.x; i < ROWS * V; i += 32 * W) {
-      float v = 0.0f;
+    for (int i = 4 * threadIdx.x; i < ROWS * PITCH; i += 128 * W) {
+      float4 v = *reinterpret_cast<const float4*>(slab + ROWS * PITCH + i);
 #pragma unroll
-      for (int w = 1; w <= W; ++w) v += slab[w * ROWS * V + i];
-      slab[i] = v;
+      for (int w = 2; w <= W; ++w) {
+        const float4 u = *reinterpret_cast<const float4*>(slab + w * ROWS * PITCH + i);
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+      }
+      *reinterpret_cast<float4*>(slab + i) = v;
     }
     __syncthreads();
   }
@@ -538,7 +542,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
   }
   const uint32_t slab_at = smem_u32(slab), max_at = smem_u32(sh->row_max), den_at = smem_u32(sh->row_den);
   for (int i = (rank * 32 * W + threadIdx.x) * 4; i < rows * V && !dead; i += ctas * 32 * W * 4) {
-    const int r = i / V, d = i % V, flat = row0 + r, head = group * a.H + flat % a.H;
+    const int r = i / V, d = i % V, at = r * PITCH + d, flat = row0 + r, head = group * a.H + flat % a.H;
     if (d >= a.R) continue;
     const float sink = a.sink ? a.sink[head] * 1.4426950408889634f : -INFINITY;
     float m = sink, sum = 0.0f, v[4] = {};
@@ -548,13 +552,13 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
       const float g = mk == -INFINITY ? (dk == 0.0f ? 0.0f : 1.0f) : a4_exp2(mk - m);      // a part with no key has no weight
       sum = g * dk;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = g * slab[i + e];
+      for (int e = 0; e < 4; ++e) v[e] = g * slab[at + e];
     } else {
       for (uint32_t k = 0; k < ctas; ++k) m = fmaxf(m, ld_cluster(mapa_shared(max_at + 4 * r, k)));
       for (uint32_t k = 0; k < ctas; ++k) {
         const float mk = ld_cluster(mapa_shared(max_at + 4 * r, k)), dk = ld_cluster(mapa_shared(den_at + 4 * r, k));
         const float g = mk == -INFINITY ? (dk == 0.0f ? 0.0f : 1.0f) : a4_exp2(mk - m);
-        const uint32_t from = mapa_shared(slab_at + 4 * i, k);
+        const uint32_t from = mapa_shared(slab_at + 4 * at, k);
         sum += g * dk;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += g * ld_cluster(from + 4 * e);

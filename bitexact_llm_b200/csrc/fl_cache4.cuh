@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(s4_threads(ROWS)) fl_store4_kernel(const Store
 
 // The entries that the cache holds at `slot`: k T [M][G][dim], v T [M][G][vdim]; slots outside the cache give zeros. Half a warp per row and
 // head, a lane for eight entries (of a value: four bytes 64 apart, entries 8 apart in their halves). A CTA has rows of one head: they share the sectors of the
-// values' bytes where their slots are neighbours: 8192 rows of 8 heads in 13 us behind the store, 27 with the heads of a row together.
+// values' bytes where their slots are neighbours: 8192 rows of 8 heads in 13 us behind the store, 24 with the heads of a row together.
 constexpr int R4_ROWS = 8;                                 // of a CTA
 
 template <class T>
