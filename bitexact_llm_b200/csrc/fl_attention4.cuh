@@ -105,6 +105,9 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
 // W-th block of its CTA's keys, in a ring of its own filled by bulk copies (one per block): warps never wait for one another until
 // the end. The parts are joined through shared memory and that of the cluster in a fixed order, so there is one launch, no scratch
 // memory, and the same bits in every call.
+//
+// What bounds it: the ALU (66 %) and issue (62 %), which conversions, scales and permutes of the codes take: 64 tokens over 8192 keys of 128 + 128 entries,
+// 8 heads, in 134 us (4.6 TB/s); short contexts what a CTA does once, half of its time (256 tokens over 64 .. 1100 keys of 64 + 64: 40 us).
 constexpr int A4_STAGES = 2, A4_MAX_CLUSTER = 16, A4_ROWS_MAX = 16;
 constexpr int A4_BIAS = 14;            // weights are kept times 2^14
 
