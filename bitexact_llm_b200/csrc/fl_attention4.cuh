@@ -10,12 +10,15 @@ namespace bxf {
 // ---- any sizes, both element types: one CTA per (query row, head), products in 32 bits ----
 // A block of 64 keys at a time: two threads share a key (its scores from codes, scaled block by block of 16), then a thread owns two
 // entries of the value and half of the tokens. PagedAttn's W and R are the entries of key and value, bs the tokens of a page.
+// Codes become fp16 by the hardware's conversions, exactly; 20 tokens over 100 .. 800 keys of 128 + 128 entries, 16 heads: 38 us (123 with codes
+// taken apart by integer operations). It does not split a context: one token over 10000 keys takes 290.
 constexpr int A4_THREADS = 128;
 
 template <class T>
 __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const PagedAttn a, const Cache4 c) {
-  extern __shared__ float a4_smem[];                       // query [K], then the value's accumulators [2][V]
-  __shared__ float p[C4_TOKENS], red[2][4];
+  extern __shared__ __align__(16) float a4_smem[];                       // query [K], then the value's accumulators [2][V]
+  __shared__ __align__(16) float p[C4_TOKENS];
+  __shared__ float red[2][4];
   const int m = blockIdx.x, h = blockIdx.y, g = h / a.H, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   float *q = a4_smem, *acc = a4_smem + c.K;
   launch_next();
@@ -30,14 +33,23 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
   for (int k0 = first / C4_TOKENS * C4_TOKENS; k0 <= pos; k0 += C4_TOKENS) {
     const uint8_t* b = c.block(a.page_of(s, k0 / a.bs) * a.bs + k0 % a.bs, g);
     {
-      const int tok = tid >> 1, half = tid & 1, j0 = half * (c.K / 32);
+      const int tok = tid >> 1, half = tid & 1;
       float v = 0.0f;
-      for (int j = j0; j < j0 + c.K / 32; ++j) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(b + tok * (c.K / 2) + j * 8);
-        float part = 0.0f;
+      for (int j = half; j < c.K / 16; j += 2) {           // (every other one: the two threads' queries lie in different banks)
+        const uint2 w = *reinterpret_cast<const uint2*>(b + tok * (c.K / 2) + j * 8);
+        uint32_t codes[2][4];
+        e2m1_pairs(w.x, codes[0]);
+        e2m1_pairs(w.y, codes[1]);
+        float even = 0.0f, odd = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part = fmaf(q[j * 16 + i], c4_code(w[i / 8] >> (i % 8 * 4) & 15), part);
-        v = fmaf(part, c4_scale(b[c.key_scale(tok, j)] & 127), v);
+        for (int i = 0; i < 4; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(q + j * 16 + 4 * i);
+          const float2 c0 = __half22float2(*reinterpret_cast<const __half2*>(&codes[i / 2][i % 2 * 2]));
+          const float2 c1 = __half22float2(*reinterpret_cast<const __half2*>(&codes[i / 2][i % 2 * 2 + 1]));
+          even = fmaf(x.x, c0.x, even), odd = fmaf(x.y, c0.y, odd);
+          even = fmaf(x.z, c1.x, even), odd = fmaf(x.w, c1.y, odd);
+        }
+        v = fmaf(even + odd, c4_scale(b[c.key_scale(tok, j)] & 127), v);
       }
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       v *= __int_as_float(b[c.key_exp(tok)] << 23) * a.scale;
@@ -70,12 +82,25 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
       const uint8_t *codes = b + 36 * c.K + col * C4_TOKENS, *scales = b + 36 * c.K + 32 * c.V + j * C4_TOKENS;
       float* o = acc + half * c.V + j * 16 + col % 8;
       float lo = o[0] * corr, hi = o[8] * corr;
-      for (int t = half * 32; t < half * 32 + 32; ++t) {
-        const float w = p[t];
-        if (w == 0.0f) continue;                           // behind the last token lies whatever was there before
-        const float f = w * c4_scale(scales[t] & 127);
-        lo = fmaf(f, c4_code(codes[t] & 15), lo);
-        hi = fmaf(f, c4_code(codes[t] >> 4), hi);
+#pragma unroll
+      for (int t = half * 32; t < half * 32 + 32; t += 16) {             // (what lies behind the last token is finite and has no weight)
+        const uint4 vc = *reinterpret_cast<const uint4*>(codes + t), vs = *reinterpret_cast<const uint4*>(scales + t);
+        const uint32_t cw[4] = {vc.x, vc.y, vc.z, vc.w}, sw[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float4 w = *reinterpret_cast<const float4*>(p + t + 4 * x);
+          const float weight[4] = {w.x, w.y, w.z, w.w};
+          uint32_t e[4];
+          e2m1_pairs(cw[x], e);
+          const uint32_t f[2] = {e4m3_pair(sw[x] & 0x7f7f7f7fu), e4m3_pair(sw[x] >> 16 & 0x7f7fu)};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t v = hmul2(e[y], __byte_perm(f[y / 2], 0, y % 2 ? 0x3232 : 0x1010));           // exact
+            const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&v));
+            lo = fmaf(weight[y], z.x, lo);
+            hi = fmaf(weight[y], z.y, hi);
+          }
+        }
       }
       o[0] = lo;
       o[8] = hi;

@@ -72,14 +72,9 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 
 __device__ __forceinline__ float c4_power(int e) { return __int_as_float((e + 127) << 23); }
 
-// e4m3 byte (0 .. 127) -> its value; code 0 .. 15 -> its value.
+// e4m3 byte (0 .. 127) -> its value.
 __device__ __forceinline__ float c4_scale(int c) {
   return c >= 8 ? c == C4_NAN ? NAN : __int_as_float((c << 20) + (120 << 23)) : c * 0.001953125f;
-}
-__device__ __forceinline__ float c4_code(int c) {
-  const int m = c & 7;
-  const float v = m < 4 ? 0.5f * m : m == 7 ? 6.0f : (float)(m - 2);
-  return c & 8 ? -v : v;
 }
 
 // The smallest scale of which 6 steps reach `most` (below 2048): an estimate from below, which is one less unless it is exact (two where a
