@@ -49,8 +49,8 @@ struct Cache4 {
   __device__ __forceinline__ int value_exp(int tok) const { return 36 * (K + V) + C4_TOKENS + tok; }
 };
 
-// Four bytes of two e2m1 codes each -> four pairs of fp16. (The compiler of CUDA 12.9 gives zeros for a word that it knows to be a zero-extended
-// 16-bit load: such a one is handed over twice, in both halves.)
+// Four bytes of two e2m1 codes each -> four pairs of fp16. (Not for words that are zero-extended 16-bit loads: the compiler of CUDA 12.9
+// gives zeros for those.)
 __device__ __forceinline__ void e2m1_pairs(uint32_t w, uint32_t (&h)[4]) {
   asm("{\n\t.reg .b8 x, y, z, w;\n\t"
       "mov.b32 {x, y, z, w}, %4;\n\t"
