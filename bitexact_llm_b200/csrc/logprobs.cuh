@@ -273,7 +273,7 @@ struct LpState {
     sum.t += t;
   }
 
-  // Vectors of a row. Where no special case is met, that is floats without masked entries (a sum that is no number shows them) and int64
+  // Vectors of a row. Where no special case is met, that is floats below some 2800 without masked entries (a sum that is no number shows them) and int64
   // within 2^38 of zero and 2^32 of the reference, which then is a value at most 255 units above the largest entry, found from upper bits:
   // with fewer operations.
   template <int N>
@@ -299,7 +299,9 @@ struct LpState {
         peak = best;
         sum.shift_to(best, O::none(), a);
       }
-      // y by one fused multiply-add against the rounded product c = log2(e) m; what the rounding (off) makes of the sums is taken back
+      // y by one fused multiply-add against the rounded product c = log2(e) m; what the rounding (off) makes of the sums is taken back by
+      // the first two terms of 2^-off. |c| < 2^12 keeps off within half a unit of that, 2^-13, and the third term below 2^-28; larger
+      // references (and infinities) take exact differences.
       const float c = sum.m * LP_LOG2E, off = fmaf(sum.m, LP_LOG2E, -c), back = fmaf(off, -0.6931471805599453f, 1.0f);
       float s = 0.0f, t = 0.0f;
 #pragma unroll
@@ -308,7 +310,7 @@ struct LpState {
         s += w;
         t = fmaf(w, y, t);
       }
-      if (fabsf(t) < INFINITY) {
+      if (fabsf(c) < 4096.0f && fabsf(t) < INFINITY) {
         sum.s = fmaf(s, back, sum.s);
         sum.t = fmaf(fmaf(-off, s, t), back, sum.t);
       } else {
