@@ -1,7 +1,7 @@
 // Log probabilities of rows of logits [M, V]: log p of a given token, the entropy, the token's rank and the best `top` tokens.
 //
 // With a reference m near the maximum, d_v = l_v - m, S = sum e^d_v and T = sum d_v e^d_v:  log p(t) = d_t - ln S,  H = ln S - T / S,
-// rank(t) = 1 + #{l_v > l_t} + #{v < t : l_v = l_t}; computed with 2^ and log2. An entry that is -infinity (int64: at most -2^62) is masked: it has no
+// rank(t) = 1 + #{l_v > l_t} + #{v < t : l_v = l_t}; the sums computed with 2^ and log2. An entry that is -infinity (int64: at most -2^62) is masked: it has no
 // probability and is no alternative. int64 logits are fixed point: l_v - m is taken exactly, then as a float.
 //
 // ONE pass over the rows: every thread keeps a reference at or above its own entries so far with S and T relative to it (32 bits; they
@@ -84,7 +84,11 @@ __device__ __forceinline__ float lp_exp2(float v) {
   return r;
 }
 
-// x - m for x <= m as a float; -infinity where e^ of it is 0 anyway.
+// x - m for x <= m as a float: at any distance, and (lp_delta) as the argument of e^, -infinity where that is 0 anyway.
+__device__ __forceinline__ float lp_distance(float x, float m, const LogProbs&) { return x - m; }
+__device__ __forceinline__ float lp_distance(long long x, long long m, const LogProbs& a) {
+  return -(float)((unsigned long long)(m - x) >> a.shift) * a.scale;
+}
 __device__ __forceinline__ float lp_delta(float x, float m, const LogProbs&) { return x - m; }
 __device__ __forceinline__ float lp_delta(long long x, long long m, const LogProbs& a) {
   const unsigned long long u = (unsigned long long)(m - x) >> a.shift;
@@ -562,8 +566,9 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_kernel(const LogProbs
   lp_warp_join(all, n, none, a);
   // a row without any entry, or with NaN or +infinity among them, has no probabilities
   const bool live = all.m > none && all.s > 0.0f && all.s < INFINITY;
-  const float log_s = log2f(all.s);                        // ln p = ln 2 (y - log2 S)
-  auto log_p = [&](Val v) { return 0.6931471805599453f * (LpSums<Val>::y_of(v, all.m, a) - log_s); };
+  const float log_s = log2f(all.s);
+  // (the distance is a logarithm already: by way of log2 it would be rounded twice more; a sum rounded to below 1 makes no p above 1)
+  auto log_p = [&](Val v) { return fminf(fmaf(-0.6931471805599453f, log_s, lp_distance(v, all.m, a)), 0.0f); };
   if (tid == 0) {
     if (a.tok) {
       a.logp[m_row] = !live || !given ? NAN : mine > none ? log_p(mine) : -INFINITY;
