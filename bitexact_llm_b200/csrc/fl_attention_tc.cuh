@@ -611,7 +611,8 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
   }
 }
 
-// Joins the key splits: one CTA per query row (token, head).
+// Joins the key splits: one CTA per query row (token, head). A part without a key has the sum 0 and no accumulators; one whose sum is NaN
+// makes the row NaN, and a row that no part has a key for is 0.
 __global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn a, const float* part, int splits) {
   launch_next();
   wait_previous();
@@ -619,19 +620,20 @@ __global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn 
   const float* ml = part + splits * n * a.R;
   float mx = -INFINITY, f[LT_MAX_SPLIT], den = 0.0f;
   for (int s = 0; s < splits; ++s)
-    if (ml[(s * n + at) * 2 + 1] > 0.0f) mx = fmaxf(mx, ml[(s * n + at) * 2]);
+    if (ml[(s * n + at) * 2 + 1] != 0.0f) mx = fmaxf(mx, ml[(s * n + at) * 2]);
 #pragma unroll
   for (int s = 0; s < LT_MAX_SPLIT; ++s) {
-    f[s] = s < splits && ml[(s * n + at) * 2 + 1] > 0.0f ? exp2f(ml[(s * n + at) * 2] - mx) : 0.0f;
-    if (f[s] > 0.0f) den += f[s] * ml[(s * n + at) * 2 + 1];
+    const float sum = s < splits ? ml[(s * n + at) * 2 + 1] : 0.0f;
+    f[s] = sum != 0.0f ? exp2f(ml[(s * n + at) * 2] - mx) : 0.0f;
+    if (f[s] != 0.0f || isnan(sum)) den += f[s] * sum;
   }
-  const float inv = 1.0f / den;
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   bf16* out = static_cast<bf16*>(a.out) + at / heads * a.out_tok + at % heads * a.out_head;
   for (int d = threadIdx.x; d < a.R; d += 128) {
     float o = 0.0f;
 #pragma unroll
     for (int s = 0; s < LT_MAX_SPLIT; ++s)
-      if (f[s] > 0.0f) o += f[s] * part[(s * n + at) * a.R + d];
+      if (f[s] != 0.0f) o += f[s] * part[(s * n + at) * a.R + d];
     st(out + d, o * inv);
   }
 }

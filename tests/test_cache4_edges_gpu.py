@@ -1,0 +1,59 @@
+"""`gqa_attention4` over tiles whose keys are split over CTAs, and over what only some of its kernels meet. Tolerances: test_cache4_gpu.py."""
+
+import math
+
+import pytest
+import torch
+
+from test_cache4_gpu import attention, batch, close, rows, spec, tiles_of
+
+pytestmark = pytest.mark.gpu
+FORMS = [("bfloat16", 0), ("bfloat16", 1), ("bfloat16", 2), ("float32", 0)]
+
+
+@pytest.mark.parametrize("dtype,variant", FORMS)
+@pytest.mark.parametrize("new", [16, 3, 1])
+def test_what_is_not_a_number_is_seen_behind_a_split(new, dtype, variant):
+    """The last `new` tokens of 2500 (16 of them: a tall tile in four parts), a window that ends among them."""
+    from bitexact_llm_b200.hybrid import ops
+    n, bad_key, bad_value = 2500, 700, 2500 - (new + 1) // 2
+    sp = spec(8, 2, 128, 64, n - new // 2 - bad_key)
+    q, cache, bt, seq, pos, held = batch(sp, 64, [n], [new], dtype, 3)
+    k, v = rows(2, 2, 128, dtype, 1), rows(2, 2, 64, dtype, 2)
+    k[0, 0, 3], v[1, 1, 60] = math.nan, math.inf
+    for g, at in ((0, bad_key), (1, bad_value)):                # (the other head's row is stored again)
+        slot = torch.tensor([int(bt[0, at // 64]) * 64 + at % 64]).cuda()
+        a, b = (t.to(getattr(torch, dtype)) for t in ops.gqa_read4(cache, sp, slot, torch.float32))
+        a[0, g], b[0, g] = k[g, g].cuda(), v[g, g].cuda()
+        ops.gqa_store4(a, b, slot, cache)
+        for kept, now in zip(held[0], ops.gqa_read4(cache, sp, slot, torch.float32)):
+            kept[at] = now[0].double().cpu()
+    want, big = attention(q, sp, seq, pos, held, None)
+    bad = torch.zeros(new, 2, dtype=torch.bool)
+    bad[:, 0] = pos.cpu() - sp.window < bad_key
+    bad[:, 1] = pos.cpu() >= bad_value
+    assert bad.any(0).all() and (new < 3 or not bad.all(0).any())
+    for tiles in (None, tiles_of([new], 4)):
+        got = ops.gqa_attention4(q, sp, cache, bt, seq, pos, None, tiles, variant).view(new, 2, -1)
+        assert torch.isnan(got.cpu()[bad]).all()
+        ok = ~bad
+        close(got.cpu()[ok], want.view(new, 2, -1)[ok], big.double().expand(new, 2)[ok][:, None], dtype)
+
+
+@pytest.mark.parametrize("dtype,variant", FORMS)
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("new", [16, 3])
+def test_rows_that_see_nothing_behind_a_split(new, window, dtype, variant):
+    """Rows in front of their sequence (position -1) in a tile with others of a long one: zeros, with a sink or without."""
+    from bitexact_llm_b200.hybrid import ops
+    sp = spec(8, 2, 128, 64, window)
+    q, cache, bt, seq, pos, held = batch(sp, 64, [2500], [new], dtype, 4)
+    none = (new + 1) // 2
+    for sink in (None, torch.randn(8, generator=torch.Generator().manual_seed(1)).cuda()):
+        want, big = attention(q, sp, seq, pos, held, sink)
+        at = pos.clone()
+        at[:none] = -1
+        for tiles in (None, tiles_of([new], 4)):
+            got = ops.gqa_attention4(q, sp, cache, bt, seq, at, sink, tiles, variant)
+            assert not got[:none].any()
+            close(got[none:], want[none:], big[none:], dtype)
