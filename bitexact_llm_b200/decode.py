@@ -20,7 +20,9 @@ class Session:
     b of its cache). By default every sequence owns a run of pages for max_len tokens. With `pages`, the cache has that
     many pages for all sequences together: `feed` takes them as a sequence grows and `release` gives them back. With `on_device`
     the pool is kept on the device (`pages.DevicePages`): `step` takes pages too, without a host synchronisation, so that it
-    can be captured into a graph; what it finds (no pages left, a sequence beyond max_len) is raised by `check`."""
+    can be captured into a graph; what it finds (no pages left, a sequence beyond max_len) is raised by `check`. `feed` and `prefill`
+    raise their own errors alone, and a call of theirs that raises leaves lengths and pool as they were (what an engine that fails on the
+    way has made of recurrent states is not put back: such sequences are to be released)."""
 
     def __init__(self, eng, B, max_len, bs=None, perm_seed=None, pages=None, on_device=False):
         bs = eng.page if bs is None else bs
@@ -94,8 +96,7 @@ class Session:
             counts = torch.zeros(self.B, dtype=torch.long)
             for s, t, _ in todo:
                 counts[s] = len(t)
-            self.pool.step(counts.to(dev), int(counts.sum()))
-            self.pool.check()
+            taken = self.pool.take(counts.to(dev), int(counts.sum()))
         else:
             for s, t, n in todo:
                 self._reserve(s, n + len(t))
@@ -141,6 +142,8 @@ class Session:
                 row += len(t)
             if self.pool is None:
                 self.lens[both[3 * at:3 * at + len(runs)]] = both[3 * at + len(runs):]
+        if self.pool is not None:                                  # the tokens are in the cache
+            self.pool.commit(taken)
         return [o[0] if len(o) == 1 else torch.cat(o) if o else torch.empty(0, self.eng.D, device=dev) for o in out]
 
     def _slots(self, seq, pos):
@@ -178,9 +181,8 @@ class Session:
         if self.free is not None:
             for b in range(B):
                 self._reserve(b, lens_host[b])
-        if self.pool is not None:                                                  # all pages at once; the lengths advance with them
-            self.pool.step(lens, sum(lens_host))
-            self.pool.check()
+        if self.pool is not None:                                                  # all pages at once
+            taken = self.pool.take(lens, sum(lens_host))
         tile_from = 0 if tiles == "always" else self.eng.tiles_from
         step = max(1, chunk_rows // B)
         last = None
@@ -209,6 +211,8 @@ class Session:
             last[seq[fin]] = x[fin]
         if self.pool is None:
             self.lens += lens
+        else:
+            self.pool.commit(taken)
         return last
 
     @torch.no_grad()

@@ -82,13 +82,30 @@ class DevicePages:
         """One step in place: counts int64 [B] new tokens on at most `rows` rows. -> StepTables."""
         return step_tables(self.lens, counts, self.bt, self.free, self.top, self.page, rows, drop, self.lens, self.top, self.status)
 
+    def take(self, counts, rows):
+        """As `step`, but the lengths and the stack stay as they are until `commit`: pages for a call that may still fail. Raises at once
+        what this call alone found (synchronises). -> StepTables."""
+        t = step_tables(self.lens, counts, self.bt, self.free, self.top, self.page, rows)
+        _told(int(t.status))
+        return t
+
+    def commit(self, t):
+        """The state behind `take`."""
+        self.lens.copy_(t.lens)
+        self.top.copy_(t.top)
+
     def check(self):
         """Raises what a step found since the last check (synchronises)."""
         bits = int(self.status)
         self.status.zero_()
-        if bits & NO_PAGES:
-            raise MemoryError("the session has no free pages")
-        if bits & TOO_LONG:
-            raise ValueError("a sequence has more tokens than its row of the block table holds (max_len)")
-        if bits:
-            raise ValueError("a step had more new tokens than rows" if bits & TOO_MANY_ROWS else "a step's lengths or pages are not valid")
+        _told(bits)
+
+
+def _told(bits):
+    """Raises what the bits of a status say."""
+    if bits & NO_PAGES:
+        raise MemoryError("the session has no free pages")
+    if bits & TOO_LONG:
+        raise ValueError("a sequence has more tokens than its row of the block table holds (max_len)")
+    if bits:
+        raise ValueError("a step had more new tokens than rows" if bits & TOO_MANY_ROWS else "a step's lengths or pages are not valid")
