@@ -76,6 +76,7 @@ class Session:
         """The sequence is finished: its pages go back to the pool and its row may serve another one. Nothing is cleared:
         keys beyond a sequence's length carry no weight, and a recurrent state starts from zero at position 0."""
         if self.pool is not None:
+            seq = seq if torch.is_tensor(seq) else range(self.B)[seq]              # (a number outside is an IndexError, as without)
             self.pool.step(torch.zeros_like(self.lens), 0, self.rows == seq)
             return
         if self.free is not None:

@@ -145,3 +145,17 @@ def test_feed_and_prefill_that_fail_change_nothing(make):
         make(2, 16, 3).prefill(prompts)
     assert torch.equal(ses.prefill(prompts), Session(Engine(), 2, 16).prefill(prompts)) and state(ses) == ([5, 5], 0)
     ses.check()
+
+
+def test_release_takes_what_a_list_takes(make):
+    """As without a pool on the device: an index from the end, and IndexError beyond."""
+    ses = make(3, 16, 4)
+    ses.feed([(0, range(3)), (2, [7] * 8)])
+    for seq in (3, -4):
+        with pytest.raises(IndexError):
+            ses.release(seq)
+    assert state(ses) == ([3, 0, 8], 1)
+    ses.release(-1)
+    assert state(ses) == ([3, 0, 0], 3)
+    ses.release(torch.tensor(0))
+    assert state(ses) == ([0, 0, 0], 4)
