@@ -23,6 +23,11 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
   float *q = a4_smem, *acc = a4_smem + c.K;
   launch_next();
   wait_previous();
+  if (a.tiles) {                                           // rows in no tile are left as they are
+    bool mine = false;
+    for (int t = tid; t < a.ntiles; t += A4_THREADS) mine |= m >= a.tiles[3 * t + 1] && m < a.tiles[3 * t + 1] + a.tiles[3 * t + 2];
+    if (!__syncthreads_or(mine)) return;
+  }
   const T* from = static_cast<const T*>(a.q) + (((i64)g * a.M + m) * a.H + h % a.H) * a.ldq;
   for (int d = tid; d < c.K; d += A4_THREADS) q[d] = d < a.W ? ld(from + d) : 0.0f;
   for (int d = tid; d < 2 * c.V; d += A4_THREADS) acc[d] = 0.0f;

@@ -612,11 +612,18 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
 }
 
 // Joins the key splits: one CTA per query row (token, head). A part without a key has the sum 0 and no accumulators; one whose sum is NaN
-// makes the row NaN, and a row that no part has a key for is 0.
-__global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn a, const float* part, int splits) {
+// makes the row NaN, and a row that no part has a key for is 0. With tiles (of up to `tokens` tokens) blockIdx.x is (tile, token of it, head):
+// rows in no tile, or in one of fewer than min_rows query rows, have no parts and are left as they are.
+__global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn a, const float* part, int splits, int tokens, int min_rows) {
   launch_next();
   wait_previous();
-  const i64 at = blockIdx.x, heads = a.H * a.G, n = a.M * heads;
+  const i64 heads = a.H * a.G, n = a.M * heads;
+  i64 at = blockIdx.x;
+  if (a.tiles) {
+    const int *tile = a.tiles + at / (heads * tokens) * 3, nth = (int)(at / heads % tokens);
+    if (nth >= tile[2] || tile[2] * a.H < min_rows) return;
+    at = (tile[1] + nth) * heads + at % heads;
+  }
   const float* ml = part + splits * n * a.R;
   float mx = -INFINITY, f[LT_MAX_SPLIT], den = 0.0f;
   for (int s = 0; s < splits; ++s)

@@ -241,6 +241,12 @@ size_t attention_scratch_for(int M, int groups, int heads, int R) {
   return attention_scratch((i64)M * groups * heads, R, splits);
 }
 
+// (keys are split for few tiles only)
+int launch_join(const PagedAttn& a, const LatentTc& c, int tokens, cudaStream_t st) {
+  const int rows = a.tiles ? a.ntiles * tokens : a.M;
+  return launch_chained(fl_attention_join_kernel, dim3((unsigned)(rows * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits, tokens, c.min_rows);
+}
+
 template <int PARTS>
 int launch_paged_tc(const PagedAttn& a, void* scratch, size_t scratch_bytes, cudaStream_t st) {
   constexpr int SMEM_MAX = PARTS == 2 ? LT_PAIR_SMEM : 227 * 1024;
@@ -280,7 +286,7 @@ int launch_paged_tc(const PagedAttn& a, void* scratch, size_t scratch_bytes, cud
   const int rc = launch_chained(fl_paged_attention_tc_kernel<PARTS>, grid, lt_threads(PARTS), fixed + c.stages * c.cols * LT_KEYS * 128, st,
                                 0, mq, mc, a, c, Cache4{});
   if (rc != BX_OK || c.splits == 1) return rc;
-  return launch_chained(fl_attention_join_kernel, dim3((unsigned)(a.M * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits);
+  return launch_join(a, c, tokens, st);
 }
 
 int run_attention(int dtype, const PagedAttn& a, void* scratch, size_t scratch_bytes, int variant, cudaStream_t st) {
@@ -407,15 +413,15 @@ int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, voi
   const int rc = launch_chained(fl_paged_attention_tc_kernel<2, true>, dim3(a.ntiles, c.splits, c.row_blocks * a.G), lt_threads(2),
                                 fixed + c.stages * c.cols * LT_KEYS * 128, st, 0, mq, mq, a, c, c4);
   if (rc != BX_OK || c.splits == 1) return rc;
-  // it writes every row; those of short tiles get what is theirs from the kernel behind it
-  return launch_chained(fl_attention_join_kernel, dim3((unsigned)(a.M * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits);
+  return launch_join(a, c, tokens, st);
 }
 
 int run_attention4(int dtype, const PagedAttn& a, const Cache4& c, void* scratch, size_t scratch_bytes, int variant, cudaStream_t st) {
-  const bool fits = attention4_fits(dtype, c) && (!a.tiles || a.ntiles > 0) && a.G <= 65535;
+  const bool fits = attention4_fits(dtype, c) && a.G <= 65535;
   const int groups = a.H <= 8 ? 1 : 2, few = 8 * groups;                             // query rows that one warp takes
   const bool tall = a.tiles && aligned16(a.q) && a.ldq % 8 == 0;                       // (a TMA copy of the queries)
   if (variant >= 2 && !fits) return BX_ELIMIT;
+  if (a.tiles && a.ntiles == 0) return BX_OK;                                          // no row is in a tile
   if (variant != 1 && fits) {
     if (tall && variant != 2) {
       const int rc = launch_attention4_tc(a, c, few + 1, scratch, scratch_bytes, st);

@@ -57,3 +57,33 @@ def test_rows_that_see_nothing_behind_a_split(new, window, dtype, variant):
             got = ops.gqa_attention4(q, sp, cache, bt, seq, at, sink, tiles, variant)
             assert not got[:none].any()
             close(got[none:], want[none:], big[none:], dtype)
+
+
+@pytest.mark.parametrize("dtype,variant", FORMS)
+@pytest.mark.parametrize("lens,new,tiles", [([2500], [40], [[0, 5, 16]]),                                     # one tall tile in parts
+                                            ([2500], [40], [[0, 3, 2], [0, 8, 30]]),                          # a short one beside it
+                                            ([300, 90, 200], [80, 1, 60], [[0, 0, 32], [1, 80, 1], [2, 100, 32]]),
+                                            ([200], [20], [[0, 7, 1]]),
+                                            ([200], [20], [])])
+def test_rows_in_no_tile_are_left_as_they_were(lens, new, tiles, dtype, variant):
+    """Through the C entry, into an output that is filled already and has columns of its own behind the heads."""
+    from bitexact_llm_b200 import _native as nv
+    from bitexact_llm_b200.hybrid import ops
+    sp = spec(8, 2, 128, 64)
+    q, cache, bt, seq, pos, held = batch(sp, 64, lens, new, dtype, 6)
+    lib, M, wide = nv.float_lib(), sum(new), 8 * 64 + 24
+    t = torch.tensor(tiles + [[0, 0, M]], dtype=torch.int32).cuda()          # (the last one is not given: a pointer to no tiles)
+    out = torch.full((M, wide), 3.0, dtype=q.dtype, device="cuda")
+    need = lib.bxf_gqa_attention_scratch(M, 8, 2, 64)
+    scratch = torch.full((need,), 255, dtype=torch.uint8, device="cuda")     # NaN
+    rc = lib.bxf_gqa_attention4(ops.code(q), q.data_ptr(), q.shape[3], M, 8, 2, 128, 64, cache.data_ptr(), 64, cache.shape[0], bt.data_ptr(), 0,
+                                bt.stride(0), bt.shape[1], seq.data_ptr(), pos.data_ptr(), t.data_ptr(), len(tiles), 0, None, sp.scale,
+                                out.data_ptr(), wide, scratch.data_ptr(), need, variant, nv.stream())
+    nv.check(rc, "bxf_gqa_attention4")
+    mine = torch.zeros(M, dtype=torch.bool)
+    for _, row, n in tiles:
+        mine[row:row + n] = True
+    assert (out[:, 8 * 64:] == 3).all() and (out.cpu()[~mine] == 3).all()
+    want, big = attention(q, sp, seq, pos, held, None)
+    if tiles:
+        close(out[:, :8 * 64].cpu()[mine], want[mine], big[mine], dtype)
