@@ -20,10 +20,12 @@
 // K-major rows as a TMA copy would leave them, values, whose codes lie along the tokens, a K-major V^T. An entry is its code times its
 // scale times 2^(e - E), with E the largest exponent of the block's keys (it goes into the scores) or values (it goes into the weights,
 // relative to the largest exponent of the values that the row has seen; the accumulator is rescaled when that grows): exact for
-// tokens within 2^14 of the largest one; values beyond are off by 2^-36 of that one's largest entry. A token that only some rows see must not cost
+// tokens within 2^14 of the largest one. Values beyond are off by less than 2^-32 of that one's largest entry (a scale by 2^-25, times a
+// code of up to 6, and the product by 2^-25; the entry is at least 2^10). A token that only some rows see must not cost
 // the others their digits, nor a large key the scores of small ones: blocks where that could be have operands without the powers of two,
-// which then go into every score and weight on its own.
-// The queries are turned to fp16 in place, each row times a power of two, and weights are held times 2^6. It is for tiles of
+// which then go into every score and weight on its own, in 32 bits. Weights are held times 2^6 in fp16: off by 2^-12 of themselves or
+// 2^-31, the larger of the two, so a token whose power of two went into its weight is off by less than 2^-30 of the largest one's largest entry.
+// The queries are turned to fp16 in place, each row times a power of two. It is for tiles of
 // many query rows, which share that work; short tiles have the kernel of fl_attention4.cuh, and each of the two leaves the
 // other's tiles alone. (Two or four warps of their own for the operands were slower: they were a chain of latencies of 4200 cycles a
 // block, where eight warps with other work beside it take turns.)
@@ -535,13 +537,12 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
         const float e0 = exp2_fast(s[2 * k] - base), e1 = exp2_fast(s[2 * k + 1] - base);
         d0 += e0;
         d1 += e1;
-        w[k] = FOUR ? pack_half(e0, e1) : pack_bf16(e0, e1);
-      }
-      if constexpr (OWN) {
-        const uint8_t* e = block_exps + C4_TOKENS + part * KW;
-#pragma unroll
-        for (int k = 0; k < KW / 2; ++k)
-          w[k] = hmul2(w[k], pack_half(c4_power(max(min((bare ? e[2 * k] : v_exp) - E, 0), -126)), c4_power(max(min((bare ? e[2 * k + 1] : v_exp) - E, 0), -126))));
+        if constexpr (OWN) {                               // the values' power of two in 32 bits: rounded once, with the weight
+          const uint8_t* e = block_exps + C4_TOKENS + part * KW + 2 * k;
+          w[k] = pack_half(e0 * c4_power(max(min((bare ? e[0] : v_exp) - E, 0), -126)), e1 * c4_power(max(min((bare ? e[1] : v_exp) - E, 0), -126)));
+        } else {
+          w[k] = FOUR ? pack_half(e0, e1) : pack_bf16(e0, e1);
+        }
       }
       den += d0 + d1;
 #pragma unroll

@@ -87,3 +87,38 @@ def test_rows_in_no_tile_are_left_as_they_were(lens, new, tiles, dtype, variant)
     want, big = attention(q, sp, seq, pos, held, None)
     if tiles:
         close(out[:, :8 * 64].cpu()[mine], want[mine], big[mine], dtype)
+
+
+@pytest.mark.parametrize("dtype,variant", FORMS)
+@pytest.mark.parametrize("keys", [1.0, 1e6])
+@pytest.mark.parametrize("per,far", [(4, 26), (4, 20), (1, 26)])
+def test_small_values_beside_a_large_one_without_weight(per, far, keys, dtype, variant):
+    """One token's values are 2^far times the others', and no row gives it any weight: what the others lose is told by fp16's smallest step.
+
+    A tall tile keeps a weight as 2^6 w 2^(e - E) in fp16: off by at most 2^-25 where that is subnormal, so w 2^(e - E) by 2^-31. A
+    token's entries are below 2^11 in units of its own power of two, the largest token's largest entry is at least 2^10: each token adds at
+    most 2^-30 of that to a sum of weights that is at least the number of tokens that weigh 1 (all of them, here). In operands that hold the powers
+    of two, scale times 2^(e - E) is off by 2^-25, times a code of at most 6, and that product by 2^-25: 7 * 2^-25 / 2^10 < 2^-32 of it.
+    So the mean is off by less than 2^-30 of the largest token's largest entry, beside the tolerances of every row."""
+    from bitexact_llm_b200.hybrid import ops
+    sp, T, n, G = spec(2 * per, 2, 64, 64), getattr(torch, dtype), 400, 2
+    k, v = torch.zeros(n, G, 64), rows(n, G, 64, "float32", 8)
+    v = v / v.abs().amax(-1, keepdim=True)
+    large = 70
+    k[large] = -keys                                        # scores 0 for the others, below -1000 for it
+    v[large] *= 2.0 ** far
+    cache, slot = ops.gqa_cache4(sp, 8, 64, "cuda"), torch.arange(n).cuda() + 64
+    ops.gqa_store4(k.to(T).cuda(), v.to(T).cuda(), slot, cache)
+    held = [tuple(x.double().cpu() for x in ops.gqa_read4(cache, sp, slot, torch.float32))]
+    first = 30
+    M = n - first
+    q = torch.full((G, M, per, 64), 200.0).to(T).cuda()
+    bt, seq, pos = torch.arange(1, 8, dtype=torch.int32).cuda()[None], torch.zeros(M, dtype=torch.long).cuda(), torch.arange(first, n).cuda()
+    want, big = attention(q, sp, seq, pos, held, None)
+    own = held[0][1][torch.arange(n) != large].abs().amax()
+    tol = 2.0 ** -30 * big + (2.0 ** -11 * own + 2.0 ** -8 * want.abs() if dtype == "bfloat16" else 3e-5 * own)
+    for tall in (128 // per, 8 // per):
+        t = torch.tensor([[0, i, min(tall, M - i)] for i in range(0, M, tall)], dtype=torch.int32).cuda()
+        got = ops.gqa_attention4(q, sp, cache, bt, seq, pos, None, t, variant)[:, :2 * per * 64].double().cpu()
+        err = (got - want).abs()
+        assert (err <= tol).all(), float((err / tol).max())
