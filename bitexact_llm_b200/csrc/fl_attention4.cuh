@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
         for (int e = 0; e < 4; ++e) v[e] += g * ld_cluster(from + 4 * e);
       }
     }
-    if (a.sink) sum += a4_exp2(sink - m);
+    if (sink != -INFINITY) sum += a4_exp2(sink - m);       // (m is -infinity too where the row sees nothing)
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     bf16* to = static_cast<bf16*>(a.out) + (tok0 + flat / a.H) * a.out_tok + head * a.out_head + d;
     if (quads) {

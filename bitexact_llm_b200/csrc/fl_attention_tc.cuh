@@ -381,7 +381,7 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     constexpr float SHIFT = FOUR ? 6.0f : 0.0f;
     float scale = a.scale * LT_LOG2E;
     float ref = a.sink ? a.sink[head] * LT_LOG2E : -INFINITY;
-    float den = a.sink && blockIdx.y == 0 && part == 0 ? UNIT : 0.0f;
+    float den = (FOUR ? ref != -INFINITY : a.sink != nullptr) && blockIdx.y == 0 && part == 0 ? UNIT : 0.0f;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
     // ---- FOUR: the operands of a block ----

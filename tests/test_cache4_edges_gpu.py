@@ -122,3 +122,40 @@ def test_small_values_beside_a_large_one_without_weight(per, far, keys, dtype, v
         got = ops.gqa_attention4(q, sp, cache, bt, seq, pos, None, t, variant)[:, :2 * per * 64].double().cpu()
         err = (got - want).abs()
         assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype,variant", FORMS)
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("n,extra", [(2500, 1), (100, 40)])
+def test_sinks_of_no_weight(n, extra, window, dtype, variant):
+    """A sink of -infinity is none: rows are as without it, and zeros where they see nothing; the table as wide as the context or far wider."""
+    from bitexact_llm_b200.hybrid import ops
+    sp, new, none = spec(8, 2, 128, 64, window), 16, 5
+    q, cache, bt, seq, pos, held = batch(sp, 64, [n], [new], dtype, 4, extra)
+    sink = torch.randn(8, generator=torch.Generator().manual_seed(1)).cuda()
+    sink[::2] = -math.inf
+    want, big = attention(q, sp, seq, pos, held, sink)
+    for tiles in (None, tiles_of([new], 4), torch.tensor([[0, i, 1] for i in range(new)], dtype=torch.int32).cuda()):
+        got = ops.gqa_attention4(q, sp, cache, bt, seq, pos, sink, tiles, variant)
+        close(got, want, big, dtype)
+        at = pos.clone()
+        at[:none] = -1
+        got = ops.gqa_attention4(q, sp, cache, bt, seq, at, sink, tiles, variant)
+        assert not got[:none].any()
+        close(got[none:], want[none:], big[none:], dtype)
+
+
+@pytest.mark.parametrize("variant", (0, 1, 2))
+@pytest.mark.parametrize("ldq,shift", [(20, 0), (21, 0), (24, 1), (24, 4), (64, 3)])
+def test_queries_of_any_stride_and_alignment(ldq, shift, variant):
+    """Rows that no 16-byte copy can take."""
+    from bitexact_llm_b200.hybrid import ops
+    sp = spec(8, 2, 20, 30)
+    lens, new = [200, 90], [40, 3]
+    q, cache, bt, seq, pos, held = batch(sp, 64, lens, new, "bfloat16", 4)
+    want, big = attention(q, sp, seq, pos, held, None)
+    room = torch.full((q.shape[0] * q.shape[1] * q.shape[2] * ldq + shift,), 9.0, dtype=q.dtype, device="cuda")
+    wide = room[shift:].view(*q.shape[:3], ldq)
+    wide[..., :20] = q[..., :20]
+    for tiles in (None, tiles_of(new, 4)):
+        close(ops.gqa_attention4(wide, sp, cache, bt, seq, pos, None, tiles, variant)[:, :240], want, big, "bfloat16")
