@@ -89,7 +89,8 @@ __device__ __forceinline__ int c4_scale_for(float most) {
 }
 // Codes of four entries in steps of `step` (inv = about 1 / step; both 0 where the block is): the quotient, corrected by its exact
 // remainder, is the correctly rounded one, and exact where it is a tie. The entries of bf16 rows come no nearer to a tie without being
-// one than 2^-12 of it; those of 32-bit rows may round to one, and are set beside it by the sign of what remains.
+// one than 2^-12 of it. A quotient of a 32-bit row may be rounded to a tie (three significant bits: only then is the rest of it looked at, since a
+// step aside may end on one), and is set beside it by the sign of what remains.
 template <class T>
 __device__ __forceinline__ uint32_t c4_codes(const float (&y)[4], float step, float inv) {
   float q[4];
@@ -100,7 +101,7 @@ __device__ __forceinline__ uint32_t c4_codes(const float (&y)[4], float step, fl
     if constexpr (sizeof(T) == 4) {
       const float rest = fmaf(-q[k], step, y[k]);
       const int bits = __float_as_int(q[k]), outward = (rest > 0.0f) == (q[k] > 0.0f) ? 1 : -1;
-      if (rest != 0.0f && q[k] != 0.0f) q[k] = __int_as_float(bits + outward);
+      if (rest != 0.0f && q[k] != 0.0f && bits << 12 == 0) q[k] = __int_as_float(bits + outward);
     }
   }
   uint32_t c;

@@ -1,11 +1,12 @@
-"""`gqa_attention4` over tiles whose keys are split over CTAs, and over what only some of its kernels meet. Tolerances: test_cache4_gpu.py."""
+"""`gqa_attention4` over tiles whose keys are split over CTAs, and over what only some of its kernels meet (tolerances: test_cache4_gpu.py); the
+decisions of `gqa_store4` where they are closest."""
 
 import math
 
 import pytest
 import torch
 
-from test_cache4_gpu import attention, batch, close, rows, spec, tiles_of
+from test_cache4_gpu import SCALES, attention, batch, close, kept, rows, spec, tiles_of
 
 pytestmark = pytest.mark.gpu
 FORMS = [("bfloat16", 0), ("bfloat16", 1), ("bfloat16", 2), ("float32", 0)]
@@ -26,8 +27,8 @@ def test_what_is_not_a_number_is_seen_behind_a_split(new, dtype, variant):
         a, b = (t.to(getattr(torch, dtype)) for t in ops.gqa_read4(cache, sp, slot, torch.float32))
         a[0, g], b[0, g] = k[g, g].cuda(), v[g, g].cuda()
         ops.gqa_store4(a, b, slot, cache)
-        for kept, now in zip(held[0], ops.gqa_read4(cache, sp, slot, torch.float32)):
-            kept[at] = now[0].double().cpu()
+        for old, now in zip(held[0], ops.gqa_read4(cache, sp, slot, torch.float32)):
+            old[at] = now[0].double().cpu()
     want, big = attention(q, sp, seq, pos, held, None)
     bad = torch.zeros(new, 2, dtype=torch.bool)
     bad[:, 0] = pos.cpu() - sp.window < bad_key
@@ -159,3 +160,39 @@ def test_queries_of_any_stride_and_alignment(ldq, shift, variant):
     wide[..., :20] = q[..., :20]
     for tiles in (None, tiles_of(new, 4)):
         close(ops.gqa_attention4(wide, sp, cache, bt, seq, pos, None, tiles, variant)[:, :240], want, big, "bfloat16")
+
+
+@pytest.mark.parametrize("dtype", ("bfloat16", "float32"))
+@pytest.mark.parametrize("few", [True, False])
+def test_entries_beside_a_tie(few, dtype):
+    """Every scale, every tie of its steps and the numbers up to five next to it, both signs; and blocks whose largest entry is beside six steps."""
+    from bitexact_llm_b200.hybrid import ops
+    T = getattr(torch, dtype)
+
+    def beside(x):
+        """x and its neighbours: x [n] -> [n, 11]."""
+        x, out = x.to(T), []
+        for to in (torch.inf, -torch.inf):
+            y = x
+            for _ in range(5):
+                y = torch.nextafter(y, torch.full_like(y, to))
+                out.append(y)
+        return torch.stack([x, *out], 1)
+
+    scales = SCALES[8:113]                                  # up to 160: six steps are within a row whose largest magnitude is 1024 .. 2047
+    entries = beside((scales[:, None] * torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)).flatten()).view(len(scales), -1)
+    entries = torch.cat([entries, -entries], 1)
+    entries = torch.nn.functional.pad(entries, (0, -entries.shape[1] % 15)).view(len(scales), -1, 15)
+    blocks = torch.cat([(6 * scales).to(T)[:, None, None].expand(-1, entries.shape[1], 1), entries], 2).reshape(-1, 16)
+    most = torch.nn.functional.pad(beside(6 * SCALES[1:113]).reshape(-1, 1), (0, 15))
+    blocks = torch.cat([blocks, most])
+    blocks = torch.nn.functional.pad(blocks, (0, 0, 0, -len(blocks) % 31)).view(-1, 31 * 16)
+    x = torch.cat([torch.full((len(blocks), 16), 1500.0).to(T), blocks], 1)[:, None]
+    x = x.repeat(1 if few else 20, 1, 1)
+    sp, M = spec(1, 1, 512, 512), len(x)
+    assert few == (M <= 512)
+    slot = torch.arange(M).cuda() + 3
+    cache = ops.gqa_cache4(sp, M // 64 + 2, 64, "cuda")
+    ops.gqa_store4(x.cuda(), -x.cuda(), slot, cache)
+    a, b = ops.gqa_read4(cache, sp, slot, torch.float32)
+    assert torch.equal(a.double().cpu(), kept(x)) and torch.equal(b.double().cpu(), kept(-x))
