@@ -7,6 +7,10 @@
 
 namespace bxf {
 
+// Sums of weighted values are held times this until they are divided by the sum of the weights: 2^16 keys of the largest magnitude
+// (2^127) stay finite, and the smallest (2^-90) are off by 2^-18 of themselves at most.
+constexpr float A4_HEADROOM = 1.0f / 65536;
+
 // ---- any sizes, both element types: one CTA per (query row, head), products in 32 bits ----
 // A block of 64 keys at a time: two threads share a key (its scores from codes, scaled block by block of 16), then a thread owns two
 // entries of the value and half of the tokens. PagedAttn's W and R are the entries of key and value, bs the tokens of a page.
@@ -78,7 +82,7 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
     }
     const float part = warp_sum(e);
     if (lane == 0) red[1][warp] = part;
-    if (tid < C4_TOKENS) p[tid] = e == 0.0f ? 0.0f : e * __int_as_float(b[c.value_exp(tid)] << 23);
+    if (tid < C4_TOKENS) p[tid] = e == 0.0f ? 0.0f : e * (__int_as_float(b[c.value_exp(tid)] << 23) * A4_HEADROOM);
     __syncthreads();
     den = den * corr + ((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
     mx = m2;
@@ -113,7 +117,7 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
     __syncthreads();
   }
   T* o = static_cast<T*>(a.out) + m * a.out_tok + h * a.out_head;
-  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  const float inv = den == 0.0f ? 0.0f : 1.0f / A4_HEADROOM / den;
   for (int d = tid; d < a.R; d += A4_THREADS) st(o + d, (acc[d] + acc[c.V + d]) * inv);
 }
 
@@ -511,7 +515,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
     if (i + A4_STAGES < n) fetch(i + A4_STAGES);
   }
 
-  // ---- the CTA's part: rows of V outputs per warp, in units of 1 ----
+  // ---- the CTA's part: rows of V outputs per warp, times A4_HEADROOM ----
   auto together = [] {
     if constexpr (W > 1) __syncthreads();
     else __syncwarp();
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
 #pragma unroll
       for (int w = 0; w < W; ++w) m = fmaxf(m, sh->max_[w][r]);
       const float unit = E[t][h] == 0 ? 0.0f : c4_power(max(E[t][h] - 127 - A4_BIAS, -126));
-      const float g = unit * (top[t][h] == -INFINITY ? 0.0f : a4_exp2(top[t][h] - m));
+      const float g = unit * A4_HEADROOM * (top[t][h] == -INFINITY ? 0.0f : a4_exp2(top[t][h] - m));
       float* to = slab + ((W > 1 ? warp + 1 : 0) * ROWS + r) * PITCH + gid;
 #pragma unroll
       for (int j = 0; j < V / 16; ++j) {
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(32 * W, (NT == 1 ? 12 : 8) / W) fl_attention4_
       }
     }
     if (sink != -INFINITY) sum += a4_exp2(sink - m);       // (m is -infinity too where the row sees nothing)
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / A4_HEADROOM / sum;
     bf16* to = static_cast<bf16*>(a.out) + (tok0 + flat / a.H) * a.out_tok + head * a.out_head + d;
     if (quads) {
       st4(to, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);

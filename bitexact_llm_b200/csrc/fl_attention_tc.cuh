@@ -575,9 +575,9 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
     } else {
       tc_fence_after();
       const i64 n = (i64)a.M * a.H * a.G, at = (i64)token * a.H * a.G + head;
-      // outputs in units of 1: of the weights where a kernel behind joins parts
+      // outputs in units of 1; where a kernel behind joins parts, of the weights (FOUR: times A4_HEADROOM)
       const float units = FOUR && E != 0 ? c4_power(max(E - 127, -126)) : 1.0f;
-      float inv = c.splits == 1 ? units / den : units / UNIT;
+      float inv = c.splits == 1 ? units / den : units * (FOUR ? A4_HEADROOM / UNIT : 1.0f);
       if (FOUR && c.splits == 1 && den == 0.0f) inv = 0.0f;                // a row that sees nothing
       float* acc = c.part + (blockIdx.y * n + at) * a.R + v0;
       bf16* out = static_cast<bf16*>(a.out) + token * a.out_tok + head * a.out_head + v0;
@@ -614,8 +614,8 @@ fl_paged_attention_tc_kernel(const __grid_constant__ CUtensorMap mq, const __gri
 
 // Joins the key splits: one CTA per query row (token, head). A part without a key has the sum 0 and no accumulators; one whose sum is NaN
 // makes the row NaN, and a row that no part has a key for is 0. With tiles (of up to `tokens` tokens) blockIdx.x is (tile, token of it, head):
-// rows in no tile, or in one of fewer than min_rows query rows, have no parts and are left as they are.
-__global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn a, const float* part, int splits, int tokens, int min_rows) {
+// rows in no tile, or in one of fewer than min_rows query rows, have no parts and are left as they are. unit: of the accumulators.
+__global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn a, const float* part, int splits, int tokens, int min_rows, float unit) {
   launch_next();
   wait_previous();
   const i64 heads = a.H * a.G, n = a.M * heads;
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(128) fl_attention_join_kernel(const PagedAttn 
     f[s] = sum != 0.0f ? exp2f(ml[(s * n + at) * 2] - mx) : 0.0f;
     if (f[s] != 0.0f || isnan(sum)) den += f[s] * sum;
   }
-  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  const float inv = den == 0.0f ? 0.0f : unit / den;
   bf16* out = static_cast<bf16*>(a.out) + at / heads * a.out_tok + at % heads * a.out_head;
   for (int d = threadIdx.x; d < a.R; d += 128) {
     float o = 0.0f;

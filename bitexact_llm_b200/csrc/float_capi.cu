@@ -242,9 +242,9 @@ size_t attention_scratch_for(int M, int groups, int heads, int R) {
 }
 
 // (keys are split for few tiles only)
-int launch_join(const PagedAttn& a, const LatentTc& c, int tokens, cudaStream_t st) {
+int launch_join(const PagedAttn& a, const LatentTc& c, int tokens, float unit, cudaStream_t st) {
   const int rows = a.tiles ? a.ntiles * tokens : a.M;
-  return launch_chained(fl_attention_join_kernel, dim3((unsigned)(rows * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits, tokens, c.min_rows);
+  return launch_chained(fl_attention_join_kernel, dim3((unsigned)(rows * a.H * a.G)), 128, 0, st, 0, a, c.part, c.splits, tokens, c.min_rows, unit);
 }
 
 template <int PARTS>
@@ -286,7 +286,7 @@ int launch_paged_tc(const PagedAttn& a, void* scratch, size_t scratch_bytes, cud
   const int rc = launch_chained(fl_paged_attention_tc_kernel<PARTS>, grid, lt_threads(PARTS), fixed + c.stages * c.cols * LT_KEYS * 128, st,
                                 0, mq, mc, a, c, Cache4{});
   if (rc != BX_OK || c.splits == 1) return rc;
-  return launch_join(a, c, tokens, st);
+  return launch_join(a, c, tokens, 1.0f, st);
 }
 
 int run_attention(int dtype, const PagedAttn& a, void* scratch, size_t scratch_bytes, int variant, cudaStream_t st) {
@@ -413,7 +413,7 @@ int launch_attention4_tc(const PagedAttn& a, const Cache4& c4, int min_rows, voi
   const int rc = launch_chained(fl_paged_attention_tc_kernel<2, true>, dim3(a.ntiles, c.splits, c.row_blocks * a.G), lt_threads(2),
                                 fixed + c.stages * c.cols * LT_KEYS * 128, st, 0, mq, mq, a, c, c4);
   if (rc != BX_OK || c.splits == 1) return rc;
-  return launch_join(a, c, tokens, st);
+  return launch_join(a, c, tokens, 1.0f / A4_HEADROOM, st);
 }
 
 int run_attention4(int dtype, const PagedAttn& a, const Cache4& c, void* scratch, size_t scratch_bytes, int variant, cudaStream_t st) {

@@ -196,3 +196,24 @@ def test_entries_beside_a_tie(few, dtype):
     ops.gqa_store4(x.cuda(), -x.cuda(), slot, cache)
     a, b = ops.gqa_read4(cache, sp, slot, torch.float32)
     assert torch.equal(a.double().cpu(), kept(x)) and torch.equal(b.double().cpu(), kept(-x))
+
+
+@pytest.mark.parametrize("dtype,variant", FORMS)
+@pytest.mark.parametrize("size", [2.0 ** 126, 2.0 ** -88])
+@pytest.mark.parametrize("n,new", [(300, 40), (2500, 16), (2500, 1)])
+def test_values_at_the_ends_of_the_range(n, new, size, dtype, variant):
+    """Many keys of about the same weight: the sum of their values is beyond 32 bits, their mean is not; and the smallest values that have all their digits."""
+    from bitexact_llm_b200.hybrid import ops
+    sp, T = spec(8, 2, 128, 64), getattr(torch, dtype)
+    g = torch.Generator().manual_seed(9)
+    k, v = torch.randn(n, 2, 128, generator=g) * 0.1, (1 + 0.9 * torch.rand(n, 2, 64, generator=g)) * size
+    v[..., ::3] *= -1
+    nblk = -(-n // 64) + 1
+    cache, slot = ops.gqa_cache4(sp, nblk + 1, 64, "cuda"), torch.arange(n).cuda() + 64
+    ops.gqa_store4(k.to(T).cuda(), v.to(T).cuda(), slot, cache)
+    held = [tuple(x.double().cpu() for x in ops.gqa_read4(cache, sp, slot, torch.float32))]
+    q = torch.randn(2, new, 4, 128, generator=g).to(T).cuda()
+    bt, seq, pos = torch.arange(1, nblk + 1, dtype=torch.int32).cuda()[None], torch.zeros(new, dtype=torch.long).cuda(), torch.arange(n - new, n).cuda()
+    want, big = attention(q, sp, seq, pos, held, None)
+    for tiles in (None, tiles_of([new], 4), torch.tensor([[0, i, 1] for i in range(new)], dtype=torch.int32).cuda()):
+        close(ops.gqa_attention4(q, sp, cache, bt, seq, pos, None, tiles, variant), want, big.double(), dtype)
