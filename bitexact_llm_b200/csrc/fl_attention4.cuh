@@ -14,7 +14,7 @@ constexpr float A4_HEADROOM = 1.0f / 65536;
 // ---- any sizes, both element types: one CTA per (query row, head), products in 32 bits ----
 // A block of 64 keys at a time: two threads share a key (its scores from codes, scaled block by block of 16), then a thread owns two
 // entries of the value and half of the tokens. PagedAttn's W and R are the entries of key and value, bs the tokens of a page.
-// Codes become fp16 by the hardware's conversions, exactly; 20 tokens over 100 .. 800 keys of 128 + 128 entries, 16 heads: 38 us (123 with codes
+// Codes become fp16 by the hardware's conversions, exactly; 20 tokens over 100 .. 800 keys of 128 + 128 entries, 16 heads: 36 us (123 with codes
 // taken apart by integer operations). It does not split a context: one token over 10000 keys takes 290.
 constexpr int A4_THREADS = 128;
 
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(A4_THREADS) fl_attention4_plain_kernel(const P
 // memory, and the same bits in every call.
 //
 // What bounds it: the ALU (66 %) and issue (62 %), which conversions, scales and permutes of the codes take: 64 tokens over 8192 keys of 128 + 128 entries,
-// 8 heads, in 134 us (4.6 TB/s); short contexts what a CTA does once, half of its time (256 tokens over 64 .. 1100 keys of 64 + 64: 40 us).
+// 8 heads, in 134 us (4.6 TB/s; 144 when the cache is another one in every call); short contexts what a CTA does once, half of its time (256 tokens over 64 .. 1100 keys of 64 + 64: 40 us).
 constexpr int A4_STAGES = 2, A4_MAX_CLUSTER = 16, A4_ROWS_MAX = 16;
 constexpr int A4_BIAS = 14;            // weights are kept times 2^14
 

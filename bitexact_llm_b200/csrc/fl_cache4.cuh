@@ -195,8 +195,8 @@ __host__ __device__ constexpr int s4_threads(int rows) { return rows < 8 ? 16 * 
 
 // ROWS rows of one head per CTA, half a warp per row. Keys go out as they are made (a row is contiguous); the bytes of values lie along the
 // tokens: with many rows they are put together in shared memory, and 16 (or 4) rows that lie in a run of slots go out as one store.
-// What bounds it is issue, at some 240 instructions for 256 entries of bf16: 8192 rows of 8 heads in 29 us (1.5 TB/s; a warp per row, in which four
-// lanes made the scale of a block, took 42).
+// What bounds it is issue, at some 240 instructions for 256 entries of bf16: 8192 rows of 8 heads in 29 us with cold caches (1.5 TB/s; 22 on the same rows
+// again; a warp per row, in which four lanes made the scale of a block, took 42). 32-bit rows: 29 on the same rows again.
 template <class T, int ROWS, int N>
 __global__ void __launch_bounds__(s4_threads(ROWS)) fl_store4_kernel(const Store4<T> a) {
   constexpr int PITCH = ROWS + 4, THREADS = s4_threads(ROWS), STEP = THREADS / 16;  // bytes of a value column of the CTA's rows; rows at a time
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(s4_threads(ROWS)) fl_store4_kernel(const Store
 
 // The entries that the cache holds at `slot`: k T [M][G][dim], v T [M][G][vdim]; slots outside the cache give zeros. Half a warp per row and
 // head, a lane for eight entries (of a value: four bytes 64 apart, entries 8 apart in their halves). A CTA has rows of one head: they share the sectors of the
-// values' bytes where their slots are neighbours: 8192 rows of 8 heads in 13 us behind the store, 24 with the heads of a row together.
+// values' bytes where their slots are neighbours: 8192 rows of 8 heads in 15 us, 24 with the heads of a row together.
 constexpr int R4_ROWS = 8;                                 // of a CTA
 
 template <class T>

@@ -14,7 +14,7 @@
 // this (ascending, constant) overflow the buffer and are read again, with the buffer cut to the best k before it can overflow.
 //
 // What bounds it (rows of 128256, one B200): bf16 the exponentials, one per entry at 16 a cycle and SM, and the issue slots around them (2000 rows in
-// 114 us, 4.5 TB/s); int64 the ALU and issue (256 rows with the best 20 in 61 us, 4.3 TB/s); fp32 the ends of short parts (700 rows, half
+// 114 us, 4.5 TB/s; 118 when the rows are others in every call; 130 where their logits are around 1e5); int64 the ALU and issue (256 rows with the best 20 in 61 us, 4.3 TB/s); fp32 the ends of short parts (700 rows, half
 // masked, with the best 5 in 100 us, 3.6 TB/s); few rows the latency of reading and joining (one row in 12 us).
 #pragma once
 

@@ -34,7 +34,7 @@ def step_tables(lens, counts, bt, free, top, page, rows, drop=None, lens_out=Non
     step has room for; drop bool [B] or None: requests that are over give their pages back first, and begin anew if they have new tokens.
 
     lens_out, top_out: where the state behind the step goes (may be lens and top; default: new tensors, so that the same call again
-    gives the same rows). status: an int32 [1] to which this call's bits are added (default: a new one). Bits: TOO_LONG, NO_PAGES,
+    gives the same rows; with drop the pages of one that is over and begins anew have changed by then). status: an int32 [1] to which this call's bits are added (default: a new one). Bits: TOO_LONG, NO_PAGES,
     TOO_MANY_ROWS, INVALID; with any of them no page changes hands and all rows are padding."""
     shape, i32 = lens.shape, torch.int32
     if lens.dim() != 1 or not (_whole(lens, shape) and _whole(counts, shape)) or lens_out is not None and not _whole(lens_out, shape):

@@ -536,12 +536,14 @@ int bx_logp_finish(const int64_t* S, const int64_t* zt, const int64_t* lnt, int6
 
 /* Log probabilities of rows of logits [M, V] (row stride ld >= V): BX_LOGITS_I64 fixed point at fr bits (0 .. 40; an entry of at most
  * -2^62 is masked), BX_LOGITS_F32, BX_LOGITS_BF16 (-infinity is masked; fr unused). With p = softmax(row):
- *   tok int64 [M] (NULL: none given; logp and rank are then not written): logp float [M] = ln p[tok] (-infinity where tok is masked,
- *     NaN where it is outside [0, V)), rank int64 [M] = 1 + the entries above tok's + the equal ones at lower indices (0 where outside)
+ *   tok int64 [M] (NULL: none given; logp and rank are then not written): logp float [M] = ln p[tok] (-infinity where tok is masked, and
+ *     only there for int64, however far it is below the best; NaN where it is outside [0, V)), rank int64 [M] = 1 + the entries above
+ *     tok's + the equal ones at lower indices (0 where outside)
  *   entropy float [M] = -sum p ln p
  *   top (0 .. BX_MAX_TOP): top_ids int64 [M, top], top_logp float [M, top], the best entries in order, equal ones by index; where a
  *     row has fewer unmasked entries the rest is (-1, -infinity).
- * A row with NaN or +infinity, or without an unmasked entry, has NaN, rank 0 and ids -1. Sums in 32 bits, the same bits in every call. */
+ * A row with NaN or +infinity, or without an unmasked entry, has NaN, rank 0 and ids -1. Differences of floats beyond 3.4e38 are -infinity.
+ * Sums in 32 bits, the same bits in every call. */
 #define BX_LOGITS_I64 0
 #define BX_LOGITS_F32 1
 #define BX_LOGITS_BF16 2

@@ -275,7 +275,9 @@ int bxf_gqa_attention(int dtype, const void* q, int64_t ldq, int M, int heads, i
  *                       rows with a slot outside the cache are left out)
  *   bxf_gqa_read4       what the cache holds at slot: k T [M, kv_heads, dim], v T [M, kv_heads, vdim] (zeros for a slot outside)
  *   bxf_gqa_attention4  as bxf_gqa_attention (scratch of bxf_gqa_attention_scratch bytes, may be NULL, used with tiles; rows in no tile are
- *                       not written); variant 0 automatic, 1 the plain kernel, 2 the kernel of single tokens for tiles too, 3 like 0, or BX_ELIMIT where it would be the plain one. */
+ *                       not written). A row that sees a key or value that is no number is NaN, one that sees nothing 0. variant 0
+ *                       automatic, 1 the plain kernel, 2 the kernel of single tokens for tiles too, 3 like 0, or BX_ELIMIT where it would be
+ *                       the plain one. */
 size_t bxf_cache4_block(int dim, int vdim);
 int bxf_gqa_store4(int dtype, const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
                    const int64_t* slot, int M, int kv_heads, int dim, int vdim, void* cache, int page, int nb, void* stream);
