@@ -87,11 +87,11 @@ __device__ __forceinline__ float lp_exp2(float v) {
 // x - m for x <= m as a float: at any distance, and (lp_delta) as the argument of e^, -infinity where that is 0 anyway.
 __device__ __forceinline__ float lp_distance(float x, float m, const LogProbs&) { return x - m; }
 __device__ __forceinline__ float lp_distance(long long x, long long m, const LogProbs& a) {
-  return -(float)((unsigned long long)(m - x) >> a.shift) * a.scale;
+  return -(float)(((unsigned long long)m - (unsigned long long)x) >> a.shift) * a.scale;
 }
 __device__ __forceinline__ float lp_delta(float x, float m, const LogProbs&) { return x - m; }
 __device__ __forceinline__ float lp_delta(long long x, long long m, const LogProbs& a) {
-  const unsigned long long u = (unsigned long long)(m - x) >> a.shift;
+  const unsigned long long u = ((unsigned long long)m - (unsigned long long)x) >> a.shift;
   return u >> 32 ? -INFINITY : -(float)(uint32_t)u * a.scale;
 }
 
